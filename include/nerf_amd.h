@@ -286,6 +286,44 @@ int nerf_adam_step(float *params, const float *grads, float *exp_avg, float *exp
                    int64_t step, double lr, double beta1, double beta2, double eps, double grad_scale,
                    nerf_stream_t stream);
 
+/* ---- learned codes: embedding lookup, layer norm, counter-based dropout -- the rows that a conditioned network puts in
+ * front of / between its layers (a latent code per view, normalised, regularised, concatenated to `view_dir`), beside the
+ * fixed encoders above.  No counterpart in the reference.  Element types: NERF_F32, NERF_BF16, NERF_F16; sums, statistics
+ * and products are fp32, each output is rounded once.  Rows need no alignment beyond their element's.  Strides are in
+ * elements.  Each call enqueues its launches on `stream` and can be captured into a graph; results do not depend on the
+ * launch (no atomics on values). */
+enum { NERF_F32 = 0, NERF_BF16 = 1, NERF_F16 = 2 };
+
+/* out (n,dim) = scale * table[ids], table (rows,dim) with row_stride; ids int32 / int64 (id_bytes 4 / 8).  An id outside
+ * [0, rows) is not dereferenced: its row is NaN. */
+int nerf_embedding(const void *table, int64_t rows, int64_t row_stride, int dtype, int64_t dim, const void *ids,
+                   int id_bytes, int64_t n, float scale, void *out, nerf_stream_t stream);
+/* g_table (rows,dim), OVERWRITTEN: scale * the sum of the rows of g_out (n,dim) by id, in the order of the batch; rows
+ * that no id names are 0.  Ids outside [0, rows) and ids equal to padding_idx (< 0: none) give nothing.
+ * workspace: nerf_embedding_backward_workspace_bytes; n < 2^31, rows < 2^31, dim <= 2^20. */
+int64_t nerf_embedding_backward_workspace_bytes(int64_t n, int64_t rows, int64_t dim, int dtype);
+int nerf_embedding_backward(const void *g_out, int dtype, int64_t n, int64_t dim, const void *ids, int id_bytes,
+                            int64_t rows, float scale, int64_t padding_idx, void *g_table, void *workspace,
+                            nerf_stream_t stream);
+
+/* y (M,C) = (x - mean) * rstd * weight + bias over rows of x (M,C), x_stride; mean, rstd (M,) fp32 may be NULL, weight and
+ * bias (C,) of w_dtype (dtype or fp32) may be NULL. */
+int nerf_layernorm(const void *x, int64_t x_stride, int dtype, int64_t M, int64_t C, const void *weight, const void *bias,
+                   int w_dtype, double eps, void *y, float *mean, float *rstd, nerf_stream_t stream);
+/* g_x (M,C) and, when non-NULL, g_weight / g_bias (C,) of w_dtype, all OVERWRITTEN; mean, rstd as the forward left them.
+ * workspace: nerf_layernorm_backward_workspace_bytes(M, C) (may be NULL when neither g_weight nor g_bias is asked for). */
+int64_t nerf_layernorm_backward_workspace_bytes(int64_t M, int64_t C);
+int nerf_layernorm_backward(const void *g_out, int64_t g_stride, const void *x, int64_t x_stride, int dtype, int64_t M,
+                            int64_t C, const void *weight, int w_dtype, const float *mean, const float *rstd, void *g_x,
+                            void *g_weight, void *g_bias, void *workspace, nerf_stream_t stream);
+
+/* out[i] = (keep ? x[i] / (1 - p) : 0) (+ residual[i]), i < n.  Element e = first + i is kept iff its 32 bits of the
+ * counter stream -- the low (e even) or high (e odd) half of the 64-bit word mix(key + (e >> 1) * 0xD1342543DE82EF95), mix
+ * as in nerf_counter_uniform -- are >= round(p * 2^32).  key_dev != NULL: the key is read from device memory instead (a
+ * captured graph sees the value of the moment).  The backward pass is the same call on g_out without a residual. */
+int nerf_dropout(const void *x, const void *residual, int dtype, int64_t n, double p, uint64_t key, const uint64_t *key_dev,
+                 int64_t first, void *out, nerf_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -645,6 +645,280 @@ def counter_uniform(key: int, first: int, count: int, device) -> torch.Tensor:
     return out
 
 
+# --------------------------------------------------------------------------- learned codes
+# Embedding lookup, layer norm and counter-based dropout over rows of fp32 / bf16 / fp16 (csrc/embedding.hip, layernorm.hip,
+# dropout.hip): what a conditioned network has beside the fixed encoders above.  Unlike `_gpu`, nothing is converted: an
+# element type the kernels do not have is refused.  Empty batches are served; every tensor of a call is on one GPU.
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}     # NERF_F32, NERF_BF16, NERF_F16
+
+
+def _rows(t: torch.Tensor, name: str) -> int:
+    """The NERF_* code of t's element type; raises for what the row kernels do not take."""
+    if not isinstance(t, torch.Tensor):
+        raise ValueError(f"{name}: expected torch.Tensor, got {type(t)}")
+    if not t.is_cuda:
+        raise RuntimeError(f"{name} must live on the GPU: the HIP path has no CPU fallback")
+    code = _DTYPES.get(t.dtype)
+    if code is None:
+        raise ValueError(f"{name}: expected float32, bfloat16 or float16, got {t.dtype}")
+    return code
+
+
+def _like(t: torch.Tensor, name: str, of: torch.Tensor, of_name: str, shape=None, dtype=None) -> torch.Tensor:
+    """t, contiguous, after checking that it is on of's GPU, of of's element type (or `dtype`) and shape (or `shape`)."""
+    if not isinstance(t, torch.Tensor):
+        raise ValueError(f"{name}: expected torch.Tensor, got {type(t)}")
+    if t.device != of.device:
+        raise ValueError(f"{name} is on {t.device}, {of_name} on {of.device}")
+    if t.dtype != (of.dtype if dtype is None else dtype):
+        raise ValueError(f"{name}: expected {of.dtype if dtype is None else dtype}, got {t.dtype}")
+    if t.shape != (of.shape if shape is None else shape):
+        raise ValueError(f"{name}: expected shape {tuple(of.shape if shape is None else shape)}, got {tuple(t.shape)}")
+    return t.contiguous()
+
+
+def _row_stride(t: torch.Tensor):
+    """(tensor, elements between rows) of t (..., C) seen as rows: a slice of the columns of a matrix is read in place,
+    anything else whose rows do not follow each other is copied."""
+    if t.is_contiguous():
+        return t, t.shape[-1]
+    if t.ndim == 2 and t.stride(1) == 1 and t.stride(0) >= t.shape[1]:
+        return t, t.stride(0)
+    return t.contiguous(), t.shape[-1]
+
+
+def _enqueue(device_index: int, what: str, fn, *args) -> None:
+    """One call of the C ABI on the current stream of that GPU."""
+    if device_index == torch.cuda.current_device():
+        rc = fn(*args, torch.cuda.current_stream().cuda_stream)
+    else:
+        with torch.cuda.device(device_index):
+            rc = fn(*args, torch.cuda.current_stream().cuda_stream)
+    if rc:
+        _lib.check(rc, what)
+
+
+def _table(table: torch.Tensor, name: str) -> int:
+    code = _rows(table, name)
+    if table.ndim != 2 or table.shape[0] < 1 or table.shape[1] < 1:
+        raise ValueError(f"{name}: expected a non-empty (rows, dim) tensor, got {tuple(table.shape)}")
+    return code
+
+
+def _id_bytes(ids: torch.Tensor, device) -> int:
+    if not isinstance(ids, torch.Tensor):
+        raise ValueError(f"ids: expected torch.Tensor, got {type(ids)}")
+    if ids.dtype not in (torch.int64, torch.int32):
+        raise ValueError(f"ids: expected int64 or int32, got {ids.dtype}")
+    if ids.device != device:
+        raise ValueError(f"ids are on {ids.device}, the rows on {device}")
+    return 8 if ids.dtype == torch.int64 else 4
+
+
+def embedding(table: torch.Tensor, ids: torch.Tensor, scale: float = 1.0) -> torch.Tensor:
+    """scale * table[ids]: table (rows, dim), ids (...) int64 / int32 -> (..., dim) of table's type.  An id outside
+    [0, rows) is never used as an address: its row is NaN (a negative id does not count from the end)."""
+    code = _table(table, "table")
+    wide = _id_bytes(ids, table.device)
+    table, stride = _row_stride(table)
+    ids = ids.contiguous()
+    rows, dim = table.shape
+    out = torch.empty((*ids.shape, dim), dtype=table.dtype, device=table.device)
+    _enqueue(table.get_device(), "nerf_embedding", _lib.load().nerf_embedding, table.data_ptr(), rows, stride, code, dim,
+             ids.data_ptr(), wide, ids.numel(), float(scale), out.data_ptr())
+    return out
+
+
+def embedding_backward(g_out: torch.Tensor, ids: torch.Tensor, num_rows: int, scale: float = 1.0,
+                       padding_idx: Optional[int] = None) -> torch.Tensor:
+    """Gradient of `embedding` for its table: (num_rows, dim) of g_out's type, the rows of g_out (..., dim) summed by id
+    (fp32, in a fixed order: the same bits every run) times `scale`, rounded once.  Ids outside [0, num_rows) and ids
+    equal to padding_idx give nothing."""
+    code = _rows(g_out, "g_out")
+    wide = _id_bytes(ids, g_out.device)
+    if g_out.ndim < 1 or g_out.shape[:-1] != ids.shape or g_out.shape[-1] < 1:
+        raise ValueError(f"g_out: expected shape {tuple(ids.shape)} + (dim,), got {tuple(g_out.shape)}")
+    num_rows, pad = int(num_rows), -1 if padding_idx is None else int(padding_idx)
+    if num_rows < 1 or (padding_idx is not None and not 0 <= pad < num_rows):
+        raise ValueError(f"num_rows {num_rows} must be positive, padding_idx {padding_idx} None or one of its rows")
+    lib = _lib.load()
+    g_out, ids = g_out.contiguous(), ids.contiguous()
+    n, dim, dev = ids.numel(), g_out.shape[-1], g_out.device
+    size = lib.nerf_embedding_backward_workspace_bytes(n, num_rows, dim, code)
+    if size < 0:
+        _lib.check(1, "nerf_embedding_backward_workspace_bytes")
+    g_table = torch.empty((num_rows, dim), dtype=g_out.dtype, device=dev)
+    ws = torch.empty((size,), dtype=torch.uint8, device=dev)
+    _enqueue(g_out.get_device(), "nerf_embedding_backward", lib.nerf_embedding_backward, g_out.data_ptr(), code, n, dim,
+             ids.data_ptr(), wide, num_rows, float(scale), pad, g_table.data_ptr(), ws.data_ptr())
+    return g_table
+
+
+class EmbeddingFunction(torch.autograd.Function):
+    """out = scale * table[ids], differentiable w.r.t. the table (a dense gradient).  apply(table, ids, scale, padding_idx)."""
+
+    @staticmethod
+    def forward(ctx, table, ids, scale=1.0, padding_idx=None):
+        ctx.num_rows, ctx.scale, ctx.padding_idx = table.shape[0], float(scale), padding_idx
+        ctx.save_for_backward(ids)
+        return embedding(table, ids, scale)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g_out):
+        (ids,) = ctx.saved_tensors
+        return embedding_backward(g_out, ids, ctx.num_rows, ctx.scale, ctx.padding_idx), None, None, None
+
+
+def _norm_weights(x: torch.Tensor, weight, bias):
+    """(weight, bias, element type of both): x's or fp32, None where absent."""
+    C, dtype = x.shape[-1], None
+    out = []
+    for name, t in (("weight", weight), ("bias", bias)):
+        if t is not None:
+            dtype = getattr(t, "dtype", None) if dtype is None else dtype
+            if dtype != x.dtype and dtype != torch.float32:
+                raise ValueError(f"{name}: expected {x.dtype} or float32, got {dtype}")
+            t = _like(t, name, x, "x", shape=(C,), dtype=dtype)
+        out.append(t)
+    return out[0], out[1], dtype or x.dtype
+
+
+def layernorm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
+              eps: float = 1e-5, want_stats: bool = False):
+    """Layer norm over the last axis of x (..., C): (x - mean) * rstd * weight + bias, of x's type; with want_stats also
+    mean and rstd (fp32, one per row), which the backward pass takes."""
+    code = _rows(x, "x")
+    if x.ndim < 1 or x.shape[-1] < 1:
+        raise ValueError(f"x: expected (..., C) with C >= 1, got {tuple(x.shape)}")
+    weight, bias, w_dtype = _norm_weights(x, weight, bias)
+    x, stride = _row_stride(x)
+    C = x.shape[-1]
+    M = x.numel() // C
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    mean = rstd = None
+    if want_stats:
+        mean = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+        rstd = torch.empty_like(mean)
+    _enqueue(x.get_device(), "nerf_layernorm", _lib.load().nerf_layernorm, x.data_ptr(), stride, code, M, C,
+             weight.data_ptr() if weight is not None else None, bias.data_ptr() if bias is not None else None,
+             _DTYPES[w_dtype], float(eps), y.data_ptr(), mean.data_ptr() if want_stats else None,
+             rstd.data_ptr() if want_stats else None)
+    return (y, mean, rstd) if want_stats else y
+
+
+def layernorm_backward(g_out: torch.Tensor, x: torch.Tensor, weight: Optional[torch.Tensor], mean: torch.Tensor,
+                       rstd: torch.Tensor, want_weight: bool = True, want_bias: bool = True):
+    """-> (g_x, g_weight | None, g_bias | None) of `layernorm`.  mean, rstd: what its want_stats returned.  The gradients
+    of weight and bias are of weight's type (x's where there is none), summed over the rows in fp32 in a fixed order."""
+    code = _rows(x, "x")
+    if x.ndim < 1 or x.shape[-1] < 1:
+        raise ValueError(f"x: expected (..., C) with C >= 1, got {tuple(x.shape)}")
+    weight, _, w_dtype = _norm_weights(x, weight, None)
+    mean = _like(mean, "mean", x, "x", shape=x.shape[:-1], dtype=torch.float32)
+    rstd = _like(rstd, "rstd", x, "x", shape=x.shape[:-1], dtype=torch.float32)
+    if g_out.shape != x.shape or g_out.dtype != x.dtype or g_out.device != x.device:
+        raise ValueError(f"g_out: expected {x.dtype} {tuple(x.shape)} on {x.device}, got {g_out.dtype} {tuple(g_out.shape)} "
+                         f"on {g_out.device}")
+    lib = _lib.load()
+    x, x_stride = _row_stride(x)
+    g_out, g_stride = _row_stride(g_out)
+    C, dev = x.shape[-1], x.device
+    M = x.numel() // C
+    g_x = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    g_weight = torch.empty((C,), dtype=w_dtype, device=dev) if want_weight else None
+    g_bias = torch.empty((C,), dtype=w_dtype, device=dev) if want_bias else None
+    ws = None
+    if want_weight or want_bias:
+        size = lib.nerf_layernorm_backward_workspace_bytes(M, C)
+        if size < 0:
+            _lib.check(1, "nerf_layernorm_backward_workspace_bytes")
+        ws = torch.empty((size,), dtype=torch.uint8, device=dev)
+    _enqueue(x.get_device(), "nerf_layernorm_backward", lib.nerf_layernorm_backward, g_out.data_ptr(), g_stride, x.data_ptr(),
+             x_stride, code, M, C, weight.data_ptr() if weight is not None else None, _DTYPES[w_dtype], mean.data_ptr(),
+             rstd.data_ptr(), g_x.data_ptr(), g_weight.data_ptr() if want_weight else None,
+             g_bias.data_ptr() if want_bias else None, ws.data_ptr() if ws is not None else None)
+    return g_x, g_weight, g_bias
+
+
+class LayerNormFunction(torch.autograd.Function):
+    """y = layernorm(x, weight, bias, eps), differentiable w.r.t. all three tensors.  apply(x, weight | None, bias | None, eps)."""
+
+    @staticmethod
+    def forward(ctx, x, weight=None, bias=None, eps=1e-5):
+        y, mean, rstd = layernorm(x, weight, bias, eps, want_stats=True)
+        ctx.bias_dtype = None if bias is None else bias.dtype
+        ctx.save_for_backward(x, weight, mean, rstd)
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g_out):
+        x, weight, mean, rstd = ctx.saved_tensors
+        g_x, g_w, g_b = layernorm_backward(g_out, x, weight, mean, rstd, want_weight=any(ctx.needs_input_grad[1:2]),
+                                           want_bias=any(ctx.needs_input_grad[2:3]))
+        if g_b is not None and g_b.dtype != ctx.bias_dtype:      # an fp32 bias without a weight over 16-bit rows
+            g_b = g_b.to(ctx.bias_dtype)
+        return g_x, g_w, g_b, None
+
+
+def _dropout_key(key, device):
+    """(host key, device address | None) of an int, or of an int64 tensor of one element on `device`."""
+    if isinstance(key, torch.Tensor):
+        if key.dtype != torch.int64 or key.numel() != 1 or key.device != device:
+            raise ValueError(f"key: expected an int or one int64 on {device}, got {key.dtype} {tuple(key.shape)} on {key.device}")
+        return 0, key.data_ptr()
+    return int(key) & 0xFFFFFFFFFFFFFFFF, None
+
+
+def dropout(x: torch.Tensor, p: float, key, first: int = 0, residual: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """x with a share p of its elements set to 0 and the others divided by 1 - p, plus `residual` if given.
+
+    Which ones is a function of (key, first + flat index) alone -- bits of the same counter stream as counter_uniform's,
+    csrc/dropout.hip -- so the mask is never stored and does not depend on how a batch is cut: a shard passes the flat
+    index of its first element as `first`.  key: 64 bits, one of its own per call site and step; an int, or an int64
+    tensor of one element on x's GPU, which a captured graph reads at every replay."""
+    code = _rows(x, "x")
+    p, first = float(p), int(first)
+    if not 0.0 <= p <= 1.0:
+        raise ValueError(f"dropout: p must be in [0, 1], got {p}")
+    if not 0 <= first <= 0x7FFFFFFFFFFFFFFF - x.numel():
+        raise ValueError(f"dropout: first {first} out of range")
+    host, dev_ptr = _dropout_key(key, x.device)
+    x = x.contiguous()
+    if residual is not None:
+        residual = _like(residual, "residual", x, "x")
+    out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    _enqueue(x.get_device(), "nerf_dropout", _lib.load().nerf_dropout, x.data_ptr(),
+             residual.data_ptr() if residual is not None else None, code, x.numel(), p, host, dev_ptr, first, out.data_ptr())
+    return out
+
+
+def dropout_backward(g_out: torch.Tensor, p: float, key, first: int = 0) -> torch.Tensor:
+    """Gradient of `dropout` for x (the residual's is g_out itself): the same mask and scale, on g_out."""
+    return dropout(g_out, p, key, first)
+
+
+class DropoutFunction(torch.autograd.Function):
+    """dropout(x, p, key, first, residual), differentiable w.r.t. x and residual; keeps no mask.  A key tensor must not
+    change between the two passes."""
+
+    @staticmethod
+    def forward(ctx, x, p, key, first=0, residual=None):
+        ctx.p, ctx.first = float(p), int(first)
+        ctx.host_key = None if isinstance(key, torch.Tensor) else key
+        if ctx.host_key is None:
+            ctx.save_for_backward(key)
+        return dropout(x, p, key, first, residual)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g_out):
+        key = ctx.saved_tensors[0] if ctx.host_key is None else ctx.host_key
+        g_x = dropout_backward(g_out, ctx.p, key, ctx.first) if ctx.needs_input_grad[0] else None
+        return g_x, None, None, None, g_out if any(ctx.needs_input_grad[4:]) else None
+
+
 # --------------------------------------------------------------------------- optimizer (row f1)
 def adam_step(params: torch.Tensor, grads: torch.Tensor, exp_avg: torch.Tensor, exp_avg_sq: torch.Tensor,
               step: int, lr: float, beta1: float = 0.9, beta2: float = 0.999, eps: float = 1e-8,
