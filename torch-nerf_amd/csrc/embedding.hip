@@ -40,6 +40,25 @@ __global__ __launch_bounds__(256) void embedding_kernel(const T *__restrict__ ta
     }
 }
 
+// ------------------------------------------------------------------------------------------------ zeros
+// Rows that no id names are 0, and nobody knows which before the sort: the whole table is cleared, by workgroups that run
+// beside the first sorting launch (the clear is the larger part of a large vocabulary's gradient, and the sort keeps few
+// CUs busy).  The summing launch comes after both.
+template <typename T>
+__device__ __forceinline__ void clear(T *g_table, int64_t count, int64_t block, int64_t blocks) {
+    Row<T> zero;
+#pragma unroll
+    for (int j = 0; j < Row<T>::VEC; ++j) zero.v[j] = (T)0.0f;
+    for (int64_t at = (block * blockDim.x + threadIdx.x) * Row<T>::VEC; at < count;
+         at += blocks * blockDim.x * Row<T>::VEC)
+        nerf::store_piece(g_table + at, zero, count - at);
+}
+
+template <typename T>
+__global__ __launch_bounds__(1024) void embedding_zero_kernel(T *__restrict__ g_table, int64_t count) {
+    clear(g_table, count, blockIdx.x, gridDim.x);
+}
+
 // ------------------------------------------------------------------------------------------------ sort
 // Stable least-significant-digit radix sort of (key, position), 32 bits each.  Keys are the ids; ids that give no gradient
 // take the key `rows`, behind all others.  A digit has at most 9 bits.
@@ -49,11 +68,23 @@ __global__ __launch_bounds__(256) void embedding_kernel(const T *__restrict__ ta
 // its digit by one ballot per bit, plus the count its wavefront kept so far.
 constexpr int SORT_THREADS = 1024, SORT_WAVES = SORT_THREADS / WAVE, MAX_DIGIT_BITS = 9, MAX_BINS = 1 << MAX_DIGIT_BITS;
 constexpr int TILE_ITEMS = 4, TILE = SORT_THREADS * TILE_ITEMS;            // several workgroups
-constexpr int ONE_ITEMS = 16, ONE_TILE = SORT_THREADS * ONE_ITEMS;         // one workgroup
+constexpr int ONE_TILE = SORT_THREADS * 16;                                // one workgroup, at most
 
 __device__ __forceinline__ uint32_t sort_key(const void *ids, int wide, int64_t i, int64_t rows, int64_t padding_idx) {
     const int64_t id = load_id(ids, wide, i);
     return (uint32_t)(id >= 0 && id < rows && id != padding_idx ? id : rows);
+}
+
+// the lanes of `live` whose digit is this lane's
+__device__ __forceinline__ uint64_t same_digit(uint32_t digit, int bits, uint64_t live) {
+    uint32_t lo = (uint32_t)live, hi = (uint32_t)(live >> 32);
+    for (int b = 0; b < bits; ++b) {
+        const uint32_t mine = (uint32_t)((int32_t)(digit << (31 - b)) >> 31);       // 0 or all ones
+        const uint64_t set = __ballot(mine != 0);
+        lo &= ~((uint32_t)set ^ mine);
+        hi &= ~((uint32_t)(set >> 32) ^ mine);
+    }
+    return (uint64_t)hi << 32 | lo;
 }
 
 template <int ITEMS>
@@ -65,49 +96,58 @@ struct Tile {
 template <int ITEMS>
 __device__ __forceinline__ void rank(Tile<ITEMS> &t, int n_tile, int shift, int bits, uint32_t *counts) {
     const int wave = threadIdx.x / WAVE, lane = threadIdx.x & (WAVE - 1), bins = 1 << bits;
+    const uint64_t below = (1ull << lane) - 1;
     for (int d = threadIdx.x; d < SORT_WAVES * bins; d += SORT_THREADS) counts[d] = 0;
     __syncthreads();
     volatile uint32_t *mine = counts + wave * bins;
 #pragma unroll
     for (int k = 0; k < ITEMS; ++k) {
-        const bool live = (wave * ITEMS + k) * WAVE + lane < n_tile;
+        const int first = (wave * ITEMS + k) * WAVE;
+        if (first >= n_tile) break;
+        const bool live = first + lane < n_tile;
         const uint32_t digit = (t.key[k] >> shift) & (bins - 1);
-        uint64_t same = __ballot(live);
-        for (int b = 0; b < bits; ++b) {
-            const uint64_t set = __ballot(live && (digit >> b & 1));
-            same &= (digit >> b & 1) ? set : ~set;
-        }
+        const uint64_t same = same_digit(digit, bits, __ballot(live));
         if (live) {
             const uint32_t before = mine[digit];
-            t.place[k] = before + __popcll(same & ((1ull << lane) - 1));
+            t.place[k] = before + __popcll(same & below);
             // the first of the lanes that share the digit writes; a wavefront's LDS accesses keep their order
-            if ((same & ((1ull << lane) - 1)) == 0) mine[digit] = before + __popcll(same);
+            if ((same & below) == 0) mine[digit] = before + __popcll(same);
         }
     }
     __syncthreads();
 }
 
-// counts[w][d] <- start of (d, w) in the order (digit, wavefront), given base[d] (the digit's start) or, without one, the
-// digits of this tile alone.  totals[d] <- number of pairs with digit d.  scan: SORT_WAVES + 1 words.
-__device__ __forceinline__ void digit_starts(uint32_t *counts, int bits, uint32_t *scan, const uint32_t *base, int base_step,
-                                             uint32_t *totals, int totals_step) {
-    const int bins = 1 << bits, wave = threadIdx.x / WAVE, lane = threadIdx.x & (WAVE - 1);
-    uint32_t total = 0;
-    if ((int)threadIdx.x < bins)
-        for (int w = 0; w < SORT_WAVES; ++w) total += counts[w * bins + threadIdx.x];
-    uint32_t incl = total;
+// Exclusive prefix sum of one value per thread.  sums: SORT_WAVES words.
+__device__ __forceinline__ uint32_t block_prefix(uint32_t v, uint32_t *sums) {
+    const int wave = threadIdx.x / WAVE, lane = threadIdx.x & (WAVE - 1);
+    uint32_t incl = v;
 #pragma unroll
     for (int d = 1; d < WAVE; d <<= 1) {
         const uint32_t up = __shfl_up(incl, d, WAVE);
         if (lane >= d) incl += up;
     }
-    if (lane == WAVE - 1) scan[wave] = incl;
+    if (lane == WAVE - 1) sums[wave] = incl;
     __syncthreads();
-    uint32_t start = incl - total;
-    for (int w = 0; w < wave; ++w) start += scan[w];
+    uint32_t start = incl - v;
+    for (int w = 0; w < wave; ++w) start += sums[w];
+    return start;
+}
+
+// counts[w][d] <- place of the first pair of wavefront w with digit d.  Of one tile alone (`totals` null), or of tile
+// blockIdx.x among many: totals[d] = pairs with digit d in all tiles, before[d] = in the tiles before this one.
+__device__ __forceinline__ void digit_starts(uint32_t *counts, int bits, uint32_t *sums, const uint32_t *totals,
+                                             const uint32_t *before, int64_t before_step) {
+    const int bins = 1 << bits;
+    uint32_t total = 0;
     if ((int)threadIdx.x < bins) {
-        if (totals) totals[(int64_t)threadIdx.x * totals_step] = total;
-        if (base) start = base[(int64_t)threadIdx.x * base_step];
+        if (totals)
+            total = totals[threadIdx.x];
+        else
+            for (int w = 0; w < SORT_WAVES; ++w) total += counts[w * bins + threadIdx.x];
+    }
+    uint32_t start = block_prefix(total, sums);
+    if ((int)threadIdx.x < bins) {
+        if (totals) start += before[threadIdx.x * before_step];
         for (int w = 0; w < SORT_WAVES; ++w) {
             const uint32_t c = counts[w * bins + threadIdx.x];
             counts[w * bins + threadIdx.x] = start;
@@ -117,28 +157,42 @@ __device__ __forceinline__ void digit_starts(uint32_t *counts, int bits, uint32_
     __syncthreads();
 }
 
-// All passes in one workgroup: up to ONE_TILE pairs.  The pairs go through LDS between two passes.
+// All passes in one workgroup (the first; the others clear the table): up to 1024 x ITEMS pairs.  Between two passes the
+// pairs go through LDS.
+template <int ITEMS>
+constexpr int one_lds_bytes(int bits) {
+    return 4 * (SORT_THREADS * ITEMS + (SORT_WAVES << bits) + SORT_WAVES) + 2 * SORT_THREADS * ITEMS;
+}
+
+template <typename T, int ITEMS>
 __global__ __launch_bounds__(SORT_THREADS) void embedding_sort_one_kernel(const void *__restrict__ ids, int wide, int n,
                                                                           int64_t rows, int64_t padding_idx, int passes,
                                                                           int bits, uint32_t *__restrict__ keys,
-                                                                          uint32_t *__restrict__ order) {
+                                                                          uint32_t *__restrict__ order,
+                                                                          uint32_t *__restrict__ joins,
+                                                                          T *__restrict__ g_table, int64_t count) {
+    if (blockIdx.x > 0) {
+        clear(g_table, count, blockIdx.x - 1, gridDim.x - 1);
+        return;
+    }
     extern __shared__ uint32_t lds[];
-    uint32_t *sk = lds, *counts = sk + ONE_TILE, *scan = counts + (SORT_WAVES << bits);
-    uint16_t *sp = reinterpret_cast<uint16_t *>(scan + SORT_WAVES);
+    uint32_t *sk = lds, *counts = sk + SORT_THREADS * ITEMS, *sums = counts + (SORT_WAVES << bits);
+    uint16_t *sp = reinterpret_cast<uint16_t *>(sums + SORT_WAVES);
     const int wave = threadIdx.x / WAVE, lane = threadIdx.x & (WAVE - 1);
-    Tile<ONE_ITEMS> t;
+    if (threadIdx.x == 0) *joins = 0;
+    Tile<ITEMS> t;
 #pragma unroll
-    for (int k = 0; k < ONE_ITEMS; ++k) {
-        const int i = (wave * ONE_ITEMS + k) * WAVE + lane;
+    for (int k = 0; k < ITEMS; ++k) {
+        const int i = (wave * ITEMS + k) * WAVE + lane;
         t.key[k] = i < n ? sort_key(ids, wide, i, rows, padding_idx) : 0;
         t.pos[k] = i;
     }
     for (int p = 0; p < passes; ++p) {
         rank(t, n, p * bits, bits, counts);
-        digit_starts(counts, bits, scan, nullptr, 0, nullptr, 0);
+        digit_starts(counts, bits, sums, nullptr, nullptr, 0);
 #pragma unroll
-        for (int k = 0; k < ONE_ITEMS; ++k) {
-            const int i = (wave * ONE_ITEMS + k) * WAVE + lane;
+        for (int k = 0; k < ITEMS; ++k) {
+            const int i = (wave * ITEMS + k) * WAVE + lane;
             if (i < n) {
                 const uint32_t to = counts[(wave << bits) + ((t.key[k] >> (p * bits)) & ((1 << bits) - 1))] + t.place[k];
                 sk[to] = t.key[k];
@@ -147,22 +201,81 @@ __global__ __launch_bounds__(SORT_THREADS) void embedding_sort_one_kernel(const 
         }
         __syncthreads();
 #pragma unroll
-        for (int k = 0; k < ONE_ITEMS; ++k) {
-            const int i = (wave * ONE_ITEMS + k) * WAVE + lane;
+        for (int k = 0; k < ITEMS; ++k) {
+            const int i = (wave * ITEMS + k) * WAVE + lane;
             if (i < n) { t.key[k] = sk[i]; t.pos[k] = sp[i]; }
         }
     }
 #pragma unroll
-    for (int k = 0; k < ONE_ITEMS; ++k) {
-        const int i = (wave * ONE_ITEMS + k) * WAVE + lane;
+    for (int k = 0; k < ITEMS; ++k) {
+        const int i = (wave * ITEMS + k) * WAVE + lane;
         if (i < n) { keys[i] = t.key[k]; order[i] = t.pos[k]; }
     }
 }
 
-// One pass over many tiles: totals per (digit, tile), their scan, and the move.  `keys_in` null: the first pass reads ids.
-__device__ __forceinline__ void load_tile(Tile<TILE_ITEMS> &t, int64_t n, const void *ids, int wide, int64_t rows,
-                                          int64_t padding_idx, const uint32_t *keys_in, const uint32_t *order_in) {
+// One pass over many tiles: counts [digit][tile]; their prefix sums along the tiles and the totals of the digits, one
+// workgroup a digit; the move.  `keys_in` null: the first pass, which reads the ids (and has workgroups that clear).
+__global__ __launch_bounds__(SORT_THREADS) void embedding_sort_scan_kernel(uint32_t *__restrict__ counts, int64_t tiles,
+                                                                           uint32_t *__restrict__ totals) {
+    __shared__ uint32_t sums[2][SORT_WAVES];
+    uint32_t *row = counts + blockIdx.x * tiles, carry = 0;
+    int half = 0;
+    for (int64_t at = 0; at < tiles; at += SORT_THREADS, half ^= 1) {
+        const bool live = at + threadIdx.x < tiles;
+        const uint32_t v = live ? row[at + threadIdx.x] : 0;
+        const uint32_t start = block_prefix(v, sums[half]);
+        if (live) row[at + threadIdx.x] = carry + start;
+        for (int w = 0; w < SORT_WAVES; ++w) carry += sums[half][w];
+    }
+    if (threadIdx.x == 0) totals[blockIdx.x] = carry;
+}
+
+template <typename T>
+__global__ __launch_bounds__(SORT_THREADS) void embedding_sort_count_kernel(const void *__restrict__ ids, int wide, int64_t n,
+                                                                            int64_t rows, int64_t padding_idx,
+                                                                            const uint32_t *__restrict__ keys_in, int shift,
+                                                                            int bits, int64_t tiles,
+                                                                            uint32_t *__restrict__ counts,
+                                                                            uint32_t *__restrict__ joins,
+                                                                            T *__restrict__ g_table, int64_t count) {
+    if (blockIdx.x >= tiles) {
+        clear(g_table, count, blockIdx.x - tiles, gridDim.x - tiles);
+        return;
+    }
+    __shared__ uint32_t mine[MAX_BINS];
+    const int bins = 1 << bits, wave = threadIdx.x / WAVE, lane = threadIdx.x & (WAVE - 1);
+    if (blockIdx.x == 0 && threadIdx.x == 0) *joins = 0;
+    for (int d = threadIdx.x; d < bins; d += SORT_THREADS) mine[d] = 0;
+    __syncthreads();
+    uint32_t key[TILE_ITEMS];
+#pragma unroll
+    for (int k = 0; k < TILE_ITEMS; ++k) {
+        const int64_t i = (int64_t)blockIdx.x * TILE + (wave * TILE_ITEMS + k) * WAVE + lane;
+        key[k] = i >= n ? 0 : keys_in ? keys_in[i] : sort_key(ids, wide, i, rows, padding_idx);
+    }
+#pragma unroll
+    for (int k = 0; k < TILE_ITEMS; ++k) {
+        const int64_t i = (int64_t)blockIdx.x * TILE + (wave * TILE_ITEMS + k) * WAVE + lane;
+        const uint32_t digit = (key[k] >> shift) & (bins - 1);
+        const uint64_t same = same_digit(digit, bits, __ballot(i < n));
+        // one addition per digit and wavefront; counts: the order does not matter
+        if (i < n && (same & ((1ull << lane) - 1)) == 0) atomicAdd(&mine[digit], (uint32_t)__popcll(same));
+    }
+    __syncthreads();
+    for (int d = threadIdx.x; d < bins; d += SORT_THREADS) counts[(int64_t)d * tiles + blockIdx.x] = mine[d];
+}
+
+__global__ __launch_bounds__(SORT_THREADS) void embedding_sort_move_kernel(const void *__restrict__ ids, int wide, int64_t n,
+                                                                           int64_t rows, int64_t padding_idx,
+                                                                           const uint32_t *__restrict__ keys_in,
+                                                                           const uint32_t *__restrict__ order_in, int shift,
+                                                                           int bits, const uint32_t *__restrict__ totals,
+                                                                           const uint32_t *__restrict__ before,
+                                                                           uint32_t *__restrict__ keys,
+                                                                           uint32_t *__restrict__ order) {
+    __shared__ uint32_t counts[SORT_WAVES * MAX_BINS], sums[SORT_WAVES];
     const int wave = threadIdx.x / WAVE, lane = threadIdx.x & (WAVE - 1);
+    Tile<TILE_ITEMS> t;
 #pragma unroll
     for (int k = 0; k < TILE_ITEMS; ++k) {
         const int64_t i = (int64_t)blockIdx.x * TILE + (wave * TILE_ITEMS + k) * WAVE + lane;
@@ -172,67 +285,9 @@ __device__ __forceinline__ void load_tile(Tile<TILE_ITEMS> &t, int64_t n, const 
             t.pos[k] = keys_in ? order_in[i] : (uint32_t)i;
         }
     }
-}
-
-__global__ __launch_bounds__(SORT_THREADS) void embedding_sort_count_kernel(const void *__restrict__ ids, int wide, int64_t n,
-                                                                            int64_t rows, int64_t padding_idx,
-                                                                            const uint32_t *__restrict__ keys_in, int shift,
-                                                                            int bits, uint32_t *__restrict__ totals) {
-    __shared__ uint32_t counts[MAX_BINS];
-    const int bins = 1 << bits;
-    for (int d = threadIdx.x; d < bins; d += SORT_THREADS) counts[d] = 0;
-    __syncthreads();
-    Tile<TILE_ITEMS> t;
-    load_tile(t, n, ids, wide, rows, padding_idx, keys_in, keys_in);
-    const int wave = threadIdx.x / WAVE, lane = threadIdx.x & (WAVE - 1);
-#pragma unroll
-    for (int k = 0; k < TILE_ITEMS; ++k) {
-        const int64_t i = (int64_t)blockIdx.x * TILE + (wave * TILE_ITEMS + k) * WAVE + lane;
-        if (i < n) atomicAdd(&counts[(t.key[k] >> shift) & (bins - 1)], 1u);   // a count: the order does not matter
-    }
-    __syncthreads();
-    for (int d = threadIdx.x; d < bins; d += SORT_THREADS) totals[(int64_t)d * gridDim.x + blockIdx.x] = counts[d];
-}
-
-// totals <- their exclusive prefix sums, one workgroup
-__global__ __launch_bounds__(SORT_THREADS) void embedding_sort_scan_kernel(uint32_t *__restrict__ totals, int64_t count) {
-    __shared__ uint32_t sums[SORT_WAVES];
-    const int wave = threadIdx.x / WAVE, lane = threadIdx.x & (WAVE - 1);
-    const int64_t per = (count + SORT_THREADS - 1) / SORT_THREADS;
-    const int64_t lo = per * threadIdx.x < count ? per * threadIdx.x : count, hi = lo + per < count ? lo + per : count;
-    uint32_t total = 0;
-    for (int64_t i = lo; i < hi; ++i) total += totals[i];
-    uint32_t incl = total;
-#pragma unroll
-    for (int d = 1; d < WAVE; d <<= 1) {
-        const uint32_t up = __shfl_up(incl, d, WAVE);
-        if (lane >= d) incl += up;
-    }
-    if (lane == WAVE - 1) sums[wave] = incl;
-    __syncthreads();
-    uint32_t run = incl - total;
-    for (int w = 0; w < wave; ++w) run += sums[w];
-    for (int64_t i = lo; i < hi; ++i) {
-        const uint32_t c = totals[i];
-        totals[i] = run;
-        run += c;
-    }
-}
-
-__global__ __launch_bounds__(SORT_THREADS) void embedding_sort_move_kernel(const void *__restrict__ ids, int wide, int64_t n,
-                                                                           int64_t rows, int64_t padding_idx,
-                                                                           const uint32_t *__restrict__ keys_in,
-                                                                           const uint32_t *__restrict__ order_in, int shift,
-                                                                           int bits, const uint32_t *__restrict__ starts,
-                                                                           uint32_t *__restrict__ keys,
-                                                                           uint32_t *__restrict__ order) {
-    __shared__ uint32_t counts[SORT_WAVES * MAX_BINS], scan[SORT_WAVES];
-    const int wave = threadIdx.x / WAVE, lane = threadIdx.x & (WAVE - 1);
-    Tile<TILE_ITEMS> t;
-    load_tile(t, n, ids, wide, rows, padding_idx, keys_in, order_in);
     const int64_t left = n - (int64_t)blockIdx.x * TILE;
     rank(t, (int)(left < TILE ? left : TILE), shift, bits, counts);
-    digit_starts(counts, bits, scan, starts + blockIdx.x, gridDim.x, nullptr, 0);
+    digit_starts(counts, bits, sums, totals, before + blockIdx.x, gridDim.x);
 #pragma unroll
     for (int k = 0; k < TILE_ITEMS; ++k) {
         if ((wave * TILE_ITEMS + k) * WAVE + lane < left) {
@@ -244,99 +299,133 @@ __global__ __launch_bounds__(SORT_THREADS) void embedding_sort_move_kernel(const
 }
 
 // ------------------------------------------------------------------------------------------------ sums
-template <typename T>
-__global__ __launch_bounds__(256) void embedding_zero_kernel(T *__restrict__ g_table, int64_t count) {
-    Row<T> zero;
-#pragma unroll
-    for (int j = 0; j < Row<T>::VEC; ++j) zero.v[j] = (T)0.0f;
-    for (int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * Row<T>::VEC; at < count;
-         at += (int64_t)gridDim.x * 256 * Row<T>::VEC)
-        nerf::store_piece(g_table + at, zero, count - at);
-}
+// A workgroup takes a span of the sorted pairs, cut into chunks: 2^shift lanes walk one chunk, a piece of the columns each.
+// An id that begins and ends in a chunk is stored by its lanes; what an id leaves in several chunks of the workgroup meets
+// in LDS, chunk after chunk.  An id that crosses workgroups leaves partial rows [workgroup][2][dim] (fp32): 0 -- the sum of
+// the id that the span begins inside of, 1 -- the sum of the id that begins in the span and goes on behind it.  The
+// workgroups of the second kind put themselves on the list of embedding_join_kernel (in any order: each is a row of its own).
+constexpr int SUM_THREADS = 256;
 
-// partial rows: [chunk][2][dim] fp32 -- 0: the sum of the id that the chunk begins inside of (up to its end, or the whole
-// chunk), 1: the sum of the id that begins in the chunk and goes on behind it
 template <typename T>
-__global__ __launch_bounds__(256) void embedding_sum_kernel(const T *__restrict__ g_out, int64_t n, int64_t dim,
-                                                            const uint32_t *__restrict__ keys,
-                                                            const uint32_t *__restrict__ order, uint32_t rows, float scale,
-                                                            int chunk, int shift, T *__restrict__ g_table,
-                                                            float *__restrict__ partial) {
+__global__ __launch_bounds__(SUM_THREADS) void embedding_sum_kernel(const T *__restrict__ g_out, int64_t n, int64_t dim,
+                                                                    const uint32_t *__restrict__ keys,
+                                                                    const uint32_t *__restrict__ order, uint32_t rows,
+                                                                    float scale, int chunk, int shift,
+                                                                    T *__restrict__ g_table, float *__restrict__ partial,
+                                                                    uint32_t *__restrict__ joins) {
     constexpr int VEC = Row<T>::VEC, AHEAD = 4;
-    const int lane = threadIdx.x & ((1 << shift) - 1);
-    const int64_t c = (int64_t)blockIdx.x * (256 >> shift) + (threadIdx.x >> shift);
-    const int64_t lo = c * chunk, hi = lo + chunk < n ? lo + chunk : n;
-    const int64_t at = ((int64_t)(blockIdx.y << shift) + lane) * VEC, left = dim - at;
-    if (lo >= n || left <= 0) return;
-    uint32_t key = keys[lo];
-    bool begins = lo == 0 || keys[lo - 1] != key;
-    float sum[VEC] = {};
-    auto flush = [&](bool ends) {
-        if (key >= rows) return;
-        if (begins && ends) {
-            Row<T> r;
+    __shared__ float part[2][SUM_THREADS * VEC];              // [head, tail][chunk][column]
+    const int group = threadIdx.x >> shift, groups = SUM_THREADS >> shift, lane = threadIdx.x & ((1 << shift) - 1);
+    const int width = VEC << shift;
+    const int64_t span = (int64_t)blockIdx.x * groups * chunk;
+    const int64_t lo = span + (int64_t)group * chunk, hi = lo + chunk < n ? lo + chunk : n;
+    const int64_t column = (int64_t)blockIdx.y * width, at = column + lane * VEC, left = dim - at;
+    if (lo < n && left > 0) {
+        uint32_t key = keys[lo];
+        bool begins = lo == 0 || keys[lo - 1] != key;
+        float sum[VEC] = {};
+        auto flush = [&](bool ends) {
+            if (key >= rows) return;
+            if (begins && ends) {
+                Row<T> r;
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) r.v[j] = (T)(sum[j] * scale);
-            nerf::store_piece(g_table + (int64_t)key * dim + at, r, left);
-        } else {
-            float *dst = partial + (c * 2 + (begins ? 1 : 0)) * dim + at;
+                for (int j = 0; j < VEC; ++j) r.v[j] = (T)(sum[j] * scale);
+                nerf::store_piece(g_table + (int64_t)key * dim + at, r, left);
+            } else {
+                float *dst = part[begins ? 1 : 0] + threadIdx.x * VEC;
 #pragma unroll
-            for (int j = 0; j < VEC; ++j)
-                if (j < left) dst[j] = sum[j];
-        }
-    };
-    for (int64_t i = lo; i < hi; i += AHEAD) {
-        uint32_t k[AHEAD];
-        Row<T> r[AHEAD];
+                for (int j = 0; j < VEC; ++j) dst[j] = sum[j];
+            }
+        };
+        for (int64_t i = lo; i < hi; i += AHEAD) {
+            uint32_t k[AHEAD];
+            Row<T> r[AHEAD];
 #pragma unroll
-        for (int u = 0; u < AHEAD; ++u) {
-            k[u] = i + u < hi ? keys[i + u] : rows;
-            r[u] = nerf::load_piece(g_out + (int64_t)(k[u] < rows ? order[i + u] : 0) * dim + at, k[u] < rows ? left : 0);
-        }
-#pragma unroll
-        for (int u = 0; u < AHEAD; ++u) {
-            if (i + u >= hi) break;
-            if (k[u] != key) {
-                flush(true);
-                key = k[u];
-                begins = true;
-#pragma unroll
-                for (int j = 0; j < VEC; ++j) sum[j] = 0.0f;
+            for (int u = 0; u < AHEAD; ++u) {
+                k[u] = i + u < hi ? keys[i + u] : rows;
+                r[u] = nerf::load_piece(g_out + (int64_t)(k[u] < rows ? order[i + u] : 0) * dim + at, k[u] < rows ? left : 0);
             }
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) sum[j] += (float)r[u].v[j];
+            for (int u = 0; u < AHEAD; ++u) {
+                if (i + u >= hi) break;
+                if (k[u] != key) {
+                    flush(true);
+                    key = k[u];
+                    begins = true;
+#pragma unroll
+                    for (int j = 0; j < VEC; ++j) sum[j] = 0.0f;
+                }
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) sum[j] += (float)r[u].v[j];
+            }
+        }
+        flush(hi >= n || keys[hi] != key);
+    }
+    __syncthreads();
+    // the chunks of this workgroup in order, one thread a column
+    for (int c = threadIdx.x; c < width && column + c < dim; c += SUM_THREADS) {
+        float sum = 0.0f;
+        bool open = false, here = false;                      // an id is open; it began in this workgroup
+        uint32_t last = rows;
+        for (int k = 0; k < groups; ++k) {
+            const int64_t a = span + (int64_t)k * chunk, b = a + chunk < n ? a + chunk : n;
+            if (a >= n) break;
+            const uint32_t first = keys[a];
+            last = keys[b - 1];
+            const bool begins = a == 0 || keys[a - 1] != first, ends = b >= n || keys[b] != last;
+            if (!begins && first < rows) {                    // the open id goes on
+                sum += part[0][k * width + c];
+                if (first != last || ends) {
+                    if (here) g_table[(int64_t)first * dim + column + c] = (T)(sum * scale);
+                    else partial[(int64_t)blockIdx.x * 2 * dim + column + c] = sum;
+                    sum = 0.0f;
+                    open = false;
+                } else {
+                    open = true;
+                }
+            }
+            if (!ends && last < rows && (first != last || begins)) {
+                sum = part[1][k * width + c];
+                open = here = true;
+            }
+        }
+        if (open) {
+            partial[((int64_t)blockIdx.x * 2 + (here ? 1 : 0)) * dim + column + c] = sum;
+            if (here && blockIdx.y == 0 && c == 0) joins[1 + atomicAdd(joins, 1u)] = blockIdx.x;
         }
     }
-    flush(hi >= n || keys[hi] != key);
 }
 
-// One workgroup per chunk (and 64 columns); it has work only where an id begins in the chunk and goes on behind it.
+// joins: [count][workgroups whose last id goes on behind them].  A workgroup takes an entry and 64 columns: the first
+// partial row and those of the spans that follow, 4 slices of them at a time.
 template <typename T>
 __global__ __launch_bounds__(256) void embedding_join_kernel(const uint32_t *__restrict__ keys, int64_t n, int64_t dim,
-                                                             uint32_t rows, float scale, int chunk,
-                                                             const float *__restrict__ partial, T *__restrict__ g_table) {
-    const int64_t c = blockIdx.x, lo = c * chunk, hi = lo + chunk;
-    if (hi >= n) return;
-    const uint32_t key = keys[hi - 1];
-    if (key >= rows || keys[hi] != key) return;
-    if (keys[lo] == key && lo > 0 && keys[lo - 1] == key) return;       // it began before
-    int64_t a = hi, b = n;                                              // first place behind the id
-    while (a < b) {
-        const int64_t m = (a + b) >> 1;
-        if (keys[m] > key) b = m; else a = m + 1;
-    }
-    const int64_t last = (a - 1) / chunk;
+                                                             float scale, int64_t span, const float *__restrict__ partial,
+                                                             const uint32_t *__restrict__ joins, T *__restrict__ g_table) {
     __shared__ float part[4][64];
     const int col = threadIdx.x & 63, s = threadIdx.x >> 6;
-    const int64_t at = (int64_t)blockIdx.y * 64 + col;
-    float sum = 0.0f;
-    if (at < dim) {
-        if (s == 0) sum = partial[(c * 2 + 1) * dim + at];
-        for (int64_t k = c + 1 + s; k <= last; k += 4) sum += partial[k * 2 * dim + at];
+    const int64_t tiles = (dim + 63) / 64, work = joins[0] * tiles;
+    for (int64_t job = blockIdx.x; job < work; job += gridDim.x) {
+        const int64_t c = joins[1 + job / tiles], at = job % tiles * 64 + col;
+        const uint32_t key = keys[(c + 1) * span];
+        int64_t a = (c + 1) * span, b = n;                              // first place behind the id
+        while (a < b) {
+            const int64_t m = (a + b) >> 1;
+            if (keys[m] > key) b = m; else a = m + 1;
+        }
+        const int64_t last = (a - 1) / span;
+        float sum = 0.0f;
+        if (at < dim) {
+            if (s == 0) sum = partial[(c * 2 + 1) * dim + at];
+#pragma unroll 8
+            for (int64_t k = c + 1 + s; k <= last; k += 4) sum += partial[k * 2 * dim + at];
+        }
+        part[s][col] = sum;
+        __syncthreads();
+        if (s == 0 && at < dim)
+            g_table[(int64_t)key * dim + at] = (T)((part[0][col] + part[1][col] + part[2][col] + part[3][col]) * scale);
+        __syncthreads();
     }
-    part[s][col] = sum;
-    __syncthreads();
-    if (s == 0 && at < dim) g_table[(int64_t)key * dim + at] = (T)((part[0][col] + part[1][col] + part[2][col] + part[3][col]) * scale);
 }
 
 // ------------------------------------------------------------------------------------------------ plan
@@ -346,8 +435,8 @@ struct Plan {
     int shift;                         // 2^shift lanes per row
     int64_t column_tiles;
     int chunk;                         // sorted pairs per lane group
-    int64_t chunks;
-    int64_t keys, order, keys2, order2, totals, partial, bytes;   // offsets in the workspace
+    int64_t spans;                     // workgroups of the sum, along the pairs
+    int64_t keys, order, keys2, order2, counts, totals, partial, joins, bytes;   // offsets in the workspace
 };
 
 int lane_shift(int64_t pieces) {
@@ -371,7 +460,8 @@ Plan plan_backward(int64_t n, int64_t rows, int64_t dim, int dtype) {
     int64_t chunk = groups > 0 ? (n + groups - 1) / groups : n;
     if (chunk < 8) chunk = 8;
     p.chunk = (int)chunk;
-    p.chunks = (n + chunk - 1) / chunk;
+    const int64_t span = chunk * (SUM_THREADS >> p.shift);
+    p.spans = (n + span - 1) / span;
     int64_t at = 0;
     auto take = [&](int64_t bytes) { const int64_t r = at; at += (bytes + 255) / 256 * 256; return r; };
     p.keys = take(4 * n);
@@ -379,8 +469,10 @@ Plan plan_backward(int64_t n, int64_t rows, int64_t dim, int dtype) {
     const bool twice = p.tiles && p.passes > 1;
     p.keys2 = take(twice ? 4 * n : 0);
     p.order2 = take(twice ? 4 * n : 0);
-    p.totals = take(p.tiles ? 4 * (p.tiles << p.bits) : 0);
-    p.partial = take(p.chunks * 2 * dim * 4);
+    p.counts = take(p.tiles ? 4 * (p.tiles << p.bits) : 0);
+    p.totals = take(p.tiles ? 4 << p.bits : 0);
+    p.partial = take(p.spans * 2 * dim * 4);
+    p.joins = take(4 * (1 + p.spans));
     p.bytes = at;
     return p;
 }
@@ -403,47 +495,63 @@ void launch_forward(const void *table, int64_t rows, int64_t row_stride, int64_t
                        static_cast<T *>(out));
 }
 
+template <typename T, int ITEMS>
+int launch_sort_one(const Plan &p, int64_t clear_blocks, const void *ids, int wide, int64_t n, int64_t rows,
+                    int64_t padding_idx, uint32_t *keys, uint32_t *order, uint32_t *joins, T *g_table, int64_t count,
+                    hipStream_t stream) {
+    static nerf::DeviceMask done;
+    auto kernel = embedding_sort_one_kernel<T, ITEMS>;
+    if (int rc = nerf::ensure_dynamic_lds(reinterpret_cast<const void *>(kernel), one_lds_bytes<ITEMS>(MAX_DIGIT_BITS), done,
+                                          "nerf_embedding_backward"))
+        return rc;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)(1 + clear_blocks)), dim3(SORT_THREADS), one_lds_bytes<ITEMS>(p.bits), stream,
+                       ids, wide, (int)n, rows, padding_idx, p.passes, p.bits, keys, order, joins, g_table, count);
+    return NERF_OK;
+}
+
 template <typename T>
 int launch_backward(const void *g_out, int dtype, int64_t n, int64_t dim, const void *ids, int wide, int64_t rows, float scale,
                     int64_t padding_idx, void *g_table, char *ws, hipStream_t stream) {
     T *gt = static_cast<T *>(g_table);
-    const int64_t count = rows * dim;
-    int64_t grid = (count + 256 * Row<T>::VEC - 1) / (256 * Row<T>::VEC);
-    hipLaunchKernelGGL(embedding_zero_kernel<T>, dim3((unsigned)(grid < 4096 ? grid : 4096)), dim3(256), 0, stream, gt, count);
-    if (n == 0) return NERF_OK;
+    const int64_t count = rows * dim, per_block = (int64_t)SORT_THREADS * Row<T>::VEC;
+    int64_t clear_blocks = (count + per_block - 1) / per_block;
+    if (clear_blocks > 1024) clear_blocks = 1024;
+    if (n == 0) {
+        hipLaunchKernelGGL(embedding_zero_kernel<T>, dim3((unsigned)clear_blocks), dim3(SORT_THREADS), 0, stream, gt, count);
+        return NERF_OK;
+    }
     const Plan p = plan_backward(n, rows, dim, dtype);
-    uint32_t *keys = reinterpret_cast<uint32_t *>(ws + p.keys), *order = reinterpret_cast<uint32_t *>(ws + p.order);
+    auto words = [&](int64_t offset) { return reinterpret_cast<uint32_t *>(ws + offset); };
+    uint32_t *keys = words(p.keys), *order = words(p.order), *joins = words(p.joins);
     float *partial = reinterpret_cast<float *>(ws + p.partial);
     if (!p.tiles) {
-        static nerf::DeviceMask done;
-        const int lds = 4 * (ONE_TILE + (SORT_WAVES << p.bits) + SORT_WAVES) + 2 * ONE_TILE;
-        if (int rc = nerf::ensure_dynamic_lds(reinterpret_cast<const void *>(embedding_sort_one_kernel), 160 * 1024, done,
-                                              "nerf_embedding_backward"))
-            return rc;
-        hipLaunchKernelGGL(embedding_sort_one_kernel, dim3(1), dim3(SORT_THREADS), lds, stream, ids, wide, (int)n, rows,
-                           padding_idx, p.passes, p.bits, keys, order);
+        auto sort = n <= SORT_THREADS       ? launch_sort_one<T, 1>
+                    : n <= SORT_THREADS * 4 ? launch_sort_one<T, 4>
+                                            : launch_sort_one<T, 16>;
+        if (int rc = sort(p, clear_blocks, ids, wide, n, rows, padding_idx, keys, order, joins, gt, count, stream)) return rc;
     } else {
-        uint32_t *totals = reinterpret_cast<uint32_t *>(ws + p.totals);
         // the last pass has to end in `keys`
-        uint32_t *k[2] = {keys, reinterpret_cast<uint32_t *>(ws + p.keys2)};
-        uint32_t *o[2] = {order, reinterpret_cast<uint32_t *>(ws + p.order2)};
+        uint32_t *k[2] = {keys, words(p.keys2)}, *o[2] = {order, words(p.order2)};
         for (int q = 0; q < p.passes; ++q) {
             const int to = (p.passes - 1 - q) & 1;
             const uint32_t *ki = q ? k[to ^ 1] : nullptr, *oi = q ? o[to ^ 1] : nullptr;
-            hipLaunchKernelGGL(embedding_sort_count_kernel, dim3((unsigned)p.tiles), dim3(SORT_THREADS), 0, stream, ids, wide,
-                               n, rows, padding_idx, ki, q * p.bits, p.bits, totals);
-            hipLaunchKernelGGL(embedding_sort_scan_kernel, dim3(1), dim3(SORT_THREADS), 0, stream, totals, p.tiles << p.bits);
+            hipLaunchKernelGGL(embedding_sort_count_kernel<T>, dim3((unsigned)(p.tiles + (q ? 0 : clear_blocks))),
+                               dim3(SORT_THREADS), 0, stream, ids, wide, n, rows, padding_idx, ki, q * p.bits, p.bits, p.tiles,
+                               words(p.counts), joins, gt, count);
+            hipLaunchKernelGGL(embedding_sort_scan_kernel, dim3(1u << p.bits), dim3(SORT_THREADS), 0, stream, words(p.counts),
+                               p.tiles, words(p.totals));
             hipLaunchKernelGGL(embedding_sort_move_kernel, dim3((unsigned)p.tiles), dim3(SORT_THREADS), 0, stream, ids, wide,
-                               n, rows, padding_idx, ki, oi, q * p.bits, p.bits, totals, k[to], o[to]);
+                               n, rows, padding_idx, ki, oi, q * p.bits, p.bits, words(p.totals), words(p.counts), k[to], o[to]);
         }
     }
-    const int64_t per = 256 >> p.shift;
-    hipLaunchKernelGGL(embedding_sum_kernel<T>, dim3((unsigned)((p.chunks + per - 1) / per), (unsigned)p.column_tiles),
-                       dim3(256), 0, stream, static_cast<const T *>(g_out), n, dim, keys, order, (uint32_t)rows, scale,
-                       p.chunk, p.shift, gt, partial);
-    if (p.chunks > 1)
-        hipLaunchKernelGGL(embedding_join_kernel<T>, dim3((unsigned)(p.chunks - 1), (unsigned)((dim + 63) / 64)), dim3(256), 0,
-                           stream, keys, n, dim, (uint32_t)rows, scale, p.chunk, partial, gt);
+    hipLaunchKernelGGL(embedding_sum_kernel<T>, dim3((unsigned)p.spans, (unsigned)p.column_tiles), dim3(SUM_THREADS), 0, stream,
+                       static_cast<const T *>(g_out), n, dim, keys, order, (uint32_t)rows, scale, p.chunk, p.shift, gt, partial,
+                       joins);
+    if (p.spans > 1) {
+        const int64_t most = (p.spans - 1) * ((dim + 63) / 64);
+        hipLaunchKernelGGL(embedding_join_kernel<T>, dim3((unsigned)(most < 1024 ? most : 1024)), dim3(256), 0, stream, keys, n,
+                           dim, scale, (int64_t)p.chunk * (SUM_THREADS >> p.shift), partial, joins, gt);
+    }
     return NERF_OK;
 }
 
