@@ -33,9 +33,9 @@ __global__ __launch_bounds__(256) void dropout_kernel(const T *__restrict__ x, c
     const int64_t pieces = (n + VEC - 1) / VEC;
     for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < pieces; i += (int64_t)gridDim.x * blockDim.x) {
         const int64_t at = i * VEC, count = n - at;
-        const Row<T> a = nerf::load_piece(x + at, count);
+        const Row<T> a = nerf::load_flat(x + at, count);
         Row<T> r;
-        if (ADD) r = nerf::load_piece(residual + at, count);
+        if (ADD) r = nerf::load_flat(residual + at, count);
         uint64_t state = key + (uint64_t)((first + at) >> 1) * GAMMA;
         uint32_t bits[2 * WORDS];
 #pragma unroll
@@ -52,7 +52,7 @@ __global__ __launch_bounds__(256) void dropout_kernel(const T *__restrict__ x, c
             const float v = keep ? (float)a.v[j] * scale : 0.0f;
             y.v[j] = (T)(ADD ? (float)r.v[j] + v : v);
         }
-        nerf::store_piece(out + at, y, count);
+        nerf::store_flat(out + at, y, count);
     }
 }
 

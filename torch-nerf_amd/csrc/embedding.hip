@@ -20,9 +20,9 @@ __device__ __forceinline__ int64_t load_id(const void *ids, int wide, int64_t i)
 }
 
 // 2^shift lanes share a row and step through its pieces
-template <typename T>
+template <typename T, bool TINY>
 __global__ __launch_bounds__(256) void embedding_kernel(const T *__restrict__ table, int64_t rows, int64_t row_stride,
-                                                        int64_t dim, const void *__restrict__ ids, int wide, int64_t n,
+                                                        int dim, const void *__restrict__ ids, int wide, int64_t n,
                                                         float scale, int shift, T *__restrict__ out) {
     constexpr int VEC = Row<T>::VEC;
     const int per = 256 >> shift, lane = threadIdx.x & ((1 << shift) - 1);
@@ -30,12 +30,12 @@ __global__ __launch_bounds__(256) void embedding_kernel(const T *__restrict__ ta
         const int64_t id = load_id(ids, wide, i);
         const bool known = id >= 0 && id < rows;
         const T *src = table + (known ? id : 0) * row_stride;
-        for (int64_t at = (int64_t)(blockIdx.y << shift) * VEC + lane * VEC; at < dim;
-             at += (int64_t)(gridDim.y << shift) * VEC) {
-            Row<T> r = nerf::load_piece(src + at, known ? dim - at : 0);
+        for (int a = (((int)blockIdx.y << shift) + lane) * VEC; a < dim; a += ((int)gridDim.y << shift) * VEC) {
+            const nerf::Place<T, TINY> at(a, dim);
+            Row<T> r = nerf::load_piece<TINY>(src, at);
 #pragma unroll
             for (int j = 0; j < VEC; ++j) r.v[j] = (T)(known ? (float)r.v[j] * scale : __builtin_nanf(""));
-            nerf::store_piece(out + i * dim + at, r, dim - at);
+            nerf::store_piece<TINY>(out + i * dim, at, r);
         }
     }
 }
@@ -43,20 +43,23 @@ __global__ __launch_bounds__(256) void embedding_kernel(const T *__restrict__ ta
 // ------------------------------------------------------------------------------------------------ zeros
 // Rows that no id names are 0, and nobody knows which before the sort: the whole table is cleared, by workgroups that run
 // beside the first sorting launch (the clear is the larger part of a large vocabulary's gradient, and the sort keeps few
-// CUs busy).  The summing launch comes after both.
+// CUs busy).  The summing launch comes after both.  A workgroup clears `per` pieces next to each other: 268 MB in 43 us
+// (6.2 TB/s); 1024 workgroups striding over the table took 60 us.
 template <typename T>
-__device__ __forceinline__ void clear(T *g_table, int64_t count, int64_t block, int64_t blocks) {
+__device__ __forceinline__ void clear(T *g_table, int64_t count, int64_t per, int64_t block) {
     Row<T> zero;
 #pragma unroll
     for (int j = 0; j < Row<T>::VEC; ++j) zero.v[j] = (T)0.0f;
-    for (int64_t at = (block * blockDim.x + threadIdx.x) * Row<T>::VEC; at < count;
-         at += blocks * blockDim.x * Row<T>::VEC)
-        nerf::store_piece(g_table + at, zero, count - at);
+    const int64_t hi = (block + 1) * per;
+    for (int64_t i = block * per + threadIdx.x; i < hi; i += blockDim.x) {
+        const int64_t at = i * Row<T>::VEC;
+        if (at < count) nerf::store_flat(g_table + at, zero, count - at);
+    }
 }
 
 template <typename T>
-__global__ __launch_bounds__(1024) void embedding_zero_kernel(T *__restrict__ g_table, int64_t count) {
-    clear(g_table, count, blockIdx.x, gridDim.x);
+__global__ __launch_bounds__(1024) void embedding_zero_kernel(T *__restrict__ g_table, int64_t count, int64_t per) {
+    clear(g_table, count, per, blockIdx.x);
 }
 
 // ------------------------------------------------------------------------------------------------ sort
@@ -169,17 +172,15 @@ __global__ __launch_bounds__(SORT_THREADS) void embedding_sort_one_kernel(const 
                                                                           int64_t rows, int64_t padding_idx, int passes,
                                                                           int bits, uint32_t *__restrict__ keys,
                                                                           uint32_t *__restrict__ order,
-                                                                          uint32_t *__restrict__ joins,
-                                                                          T *__restrict__ g_table, int64_t count) {
+                                                                          T *__restrict__ g_table, int64_t count, int64_t per) {
     if (blockIdx.x > 0) {
-        clear(g_table, count, blockIdx.x - 1, gridDim.x - 1);
+        clear(g_table, count, per, blockIdx.x - 1);
         return;
     }
     extern __shared__ uint32_t lds[];
     uint32_t *sk = lds, *counts = sk + SORT_THREADS * ITEMS, *sums = counts + (SORT_WAVES << bits);
     uint16_t *sp = reinterpret_cast<uint16_t *>(sums + SORT_WAVES);
     const int wave = threadIdx.x / WAVE, lane = threadIdx.x & (WAVE - 1);
-    if (threadIdx.x == 0) *joins = 0;
     Tile<ITEMS> t;
 #pragma unroll
     for (int k = 0; k < ITEMS; ++k) {
@@ -236,15 +237,13 @@ __global__ __launch_bounds__(SORT_THREADS) void embedding_sort_count_kernel(cons
                                                                             const uint32_t *__restrict__ keys_in, int shift,
                                                                             int bits, int64_t tiles,
                                                                             uint32_t *__restrict__ counts,
-                                                                            uint32_t *__restrict__ joins,
-                                                                            T *__restrict__ g_table, int64_t count) {
+                                                                            T *__restrict__ g_table, int64_t count, int64_t per) {
     if (blockIdx.x >= tiles) {
-        clear(g_table, count, blockIdx.x - tiles, gridDim.x - tiles);
+        clear(g_table, count, per, blockIdx.x - tiles);
         return;
     }
     __shared__ uint32_t mine[MAX_BINS];
     const int bins = 1 << bits, wave = threadIdx.x / WAVE, lane = threadIdx.x & (WAVE - 1);
-    if (blockIdx.x == 0 && threadIdx.x == 0) *joins = 0;
     for (int d = threadIdx.x; d < bins; d += SORT_THREADS) mine[d] = 0;
     __syncthreads();
     uint32_t key[TILE_ITEMS];
@@ -302,27 +301,44 @@ __global__ __launch_bounds__(SORT_THREADS) void embedding_sort_move_kernel(const
 // A workgroup takes a span of the sorted pairs, cut into chunks: 2^shift lanes walk one chunk, a piece of the columns each.
 // An id that begins and ends in a chunk is stored by its lanes; what an id leaves in several chunks of the workgroup meets
 // in LDS, chunk after chunk.  An id that crosses workgroups leaves partial rows [workgroup][2][dim] (fp32): 0 -- the sum of
-// the id that the span begins inside of, 1 -- the sum of the id that begins in the span and goes on behind it.  The
-// workgroups of the second kind put themselves on the list of embedding_join_kernel (in any order: each is a row of its own).
+// the id that the span begins inside of, 1 -- the sum of the id that begins in the span and goes on behind it, where
+// embedding_join_kernel has a row to add up (goes_on).
 constexpr int SUM_THREADS = 256;
 
-template <typename T>
-__global__ __launch_bounds__(SUM_THREADS) void embedding_sum_kernel(const T *__restrict__ g_out, int64_t n, int64_t dim,
+template <typename T, bool TINY>
+__global__ __launch_bounds__(SUM_THREADS) void embedding_sum_kernel(const T *__restrict__ g_out, int64_t n, int dim,
                                                                     const uint32_t *__restrict__ keys,
                                                                     const uint32_t *__restrict__ order, uint32_t rows,
                                                                     float scale, int chunk, int shift,
                                                                     T *__restrict__ g_table, float *__restrict__ partial,
-                                                                    uint32_t *__restrict__ joins) {
-    constexpr int VEC = Row<T>::VEC, AHEAD = 4;
+                                                                    uint32_t *__restrict__ goes_on) {
+    constexpr int VEC = Row<T>::VEC, AHEAD = 8;
+    // what a chunk has for its neighbours: HEAD -- its first id began before it; THROUGH -- and goes on behind it;
+    // TAIL -- its last id begins in it and goes on behind it
+    constexpr uint32_t HEAD = 1, THROUGH = 2, TAIL = 4;
     __shared__ float part[2][SUM_THREADS * VEC];              // [head, tail][chunk][column]
+    __shared__ uint32_t first_key[SUM_THREADS], kind[SUM_THREADS];
     const int group = threadIdx.x >> shift, groups = SUM_THREADS >> shift, lane = threadIdx.x & ((1 << shift) - 1);
     const int width = VEC << shift;
     const int64_t span = (int64_t)blockIdx.x * groups * chunk;
     const int64_t lo = span + (int64_t)group * chunk, hi = lo + chunk < n ? lo + chunk : n;
-    const int64_t column = (int64_t)blockIdx.y * width, at = column + lane * VEC, left = dim - at;
-    if (lo < n && left > 0) {
-        uint32_t key = keys[lo];
-        bool begins = lo == 0 || keys[lo - 1] != key;
+    const int column = blockIdx.y * width;
+    const nerf::Place<T, TINY> at(column + lane * VEC, dim);
+    if (lo < n && at.live()) {
+        uint32_t k[AHEAD], o[AHEAD];
+        auto fetch = [&](int64_t i) {
+#pragma unroll
+            for (int u = 0; u < AHEAD; ++u) {
+                const int64_t j = i + u < hi ? i + u : hi - 1;
+                k[u] = keys[j];
+                o[u] = order[j];
+            }
+        };
+        const uint32_t before = lo > 0 ? keys[lo - 1] : ~0u, behind = hi < n ? keys[hi] : ~0u;
+        fetch(lo);
+        uint32_t key = k[0], mark = 0;
+        bool begins = before != key;
+        const uint32_t first = key;
         float sum[VEC] = {};
         auto flush = [&](bool ends) {
             if (key >= rows) return;
@@ -330,27 +346,32 @@ __global__ __launch_bounds__(SUM_THREADS) void embedding_sum_kernel(const T *__r
                 Row<T> r;
 #pragma unroll
                 for (int j = 0; j < VEC; ++j) r.v[j] = (T)(sum[j] * scale);
-                nerf::store_piece(g_table + (int64_t)key * dim + at, r, left);
+                nerf::store_piece<TINY>(g_table + (int64_t)key * dim, at, r);
             } else {
-                float *dst = part[begins ? 1 : 0] + threadIdx.x * VEC;
+                mark |= begins ? TAIL : ends ? HEAD : HEAD | THROUGH;
+                float *dst = part[begins ? 1 : 0] + threadIdx.x * VEC - at.skip;
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) dst[j] = sum[j];
+                for (int j = 0; j < VEC; ++j)
+                    if (at.own(j)) dst[j] = sum[j];
             }
         };
         for (int64_t i = lo; i < hi; i += AHEAD) {
-            uint32_t k[AHEAD];
+            // the rows of this step are on their way while the ids of the next one are read (rows of ids that give no
+            // gradient as well: their sum goes nowhere)
             Row<T> r[AHEAD];
+            uint32_t now[AHEAD];
 #pragma unroll
             for (int u = 0; u < AHEAD; ++u) {
-                k[u] = i + u < hi ? keys[i + u] : rows;
-                r[u] = nerf::load_piece(g_out + (int64_t)(k[u] < rows ? order[i + u] : 0) * dim + at, k[u] < rows ? left : 0);
+                now[u] = k[u];
+                r[u] = nerf::load_piece<TINY>(g_out + (int64_t)o[u] * dim, at);
             }
+            if (i + AHEAD < hi) fetch(i + AHEAD);
 #pragma unroll
             for (int u = 0; u < AHEAD; ++u) {
                 if (i + u >= hi) break;
-                if (k[u] != key) {
+                if (now[u] != key) {
                     flush(true);
-                    key = k[u];
+                    key = now[u];
                     begins = true;
 #pragma unroll
                     for (int j = 0; j < VEC; ++j) sum[j] = 0.0f;
@@ -359,71 +380,77 @@ __global__ __launch_bounds__(SUM_THREADS) void embedding_sum_kernel(const T *__r
                 for (int j = 0; j < VEC; ++j) sum[j] += (float)r[u].v[j];
             }
         }
-        flush(hi >= n || keys[hi] != key);
+        flush(behind != key);
+        if (lane == 0) {
+            first_key[group] = first;
+            kind[group] = mark;
+        }
     }
     __syncthreads();
     // the chunks of this workgroup in order, one thread a column
     for (int c = threadIdx.x; c < width && column + c < dim; c += SUM_THREADS) {
         float sum = 0.0f;
         bool open = false, here = false;                      // an id is open; it began in this workgroup
-        uint32_t last = rows;
-        for (int k = 0; k < groups; ++k) {
-            const int64_t a = span + (int64_t)k * chunk, b = a + chunk < n ? a + chunk : n;
-            if (a >= n) break;
-            const uint32_t first = keys[a];
-            last = keys[b - 1];
-            const bool begins = a == 0 || keys[a - 1] != first, ends = b >= n || keys[b] != last;
-            if (!begins && first < rows) {                    // the open id goes on
-                sum += part[0][k * width + c];
-                if (first != last || ends) {
-                    if (here) g_table[(int64_t)first * dim + column + c] = (T)(sum * scale);
+        for (int g = 0; g < groups && span + (int64_t)g * chunk < n; ++g) {
+            const uint32_t mark = kind[g];
+            if (mark & HEAD) {                                // the open id goes on
+                sum += part[0][g * width + c];
+                open = true;
+                if (!(mark & THROUGH)) {
+                    if (here) g_table[(int64_t)first_key[g] * dim + column + c] = (T)(sum * scale);
                     else partial[(int64_t)blockIdx.x * 2 * dim + column + c] = sum;
-                    sum = 0.0f;
                     open = false;
-                } else {
-                    open = true;
                 }
             }
-            if (!ends && last < rows && (first != last || begins)) {
-                sum = part[1][k * width + c];
+            if (mark & TAIL) {
+                sum = part[1][g * width + c];
                 open = here = true;
             }
         }
-        if (open) {
-            partial[((int64_t)blockIdx.x * 2 + (here ? 1 : 0)) * dim + column + c] = sum;
-            if (here && blockIdx.y == 0 && c == 0) joins[1 + atomicAdd(joins, 1u)] = blockIdx.x;
-        }
+        if (open) partial[((int64_t)blockIdx.x * 2 + (here ? 1 : 0)) * dim + column + c] = sum;
+        if (blockIdx.y == 0 && c == 0) goes_on[blockIdx.x] = open && here;
     }
 }
 
-// joins: [count][workgroups whose last id goes on behind them].  A workgroup takes an entry and 64 columns: the first
-// partial row and those of the spans that follow, 4 slices of them at a time.
+// One workgroup a span and 256 columns, 4 a lane; it has work where an id begins in the span and goes on behind it: the
+// first partial row and those of the spans that follow, one wavefront every fourth of them.
 template <typename T>
 __global__ __launch_bounds__(256) void embedding_join_kernel(const uint32_t *__restrict__ keys, int64_t n, int64_t dim,
                                                              float scale, int64_t span, const float *__restrict__ partial,
-                                                             const uint32_t *__restrict__ joins, T *__restrict__ g_table) {
-    __shared__ float part[4][64];
-    const int col = threadIdx.x & 63, s = threadIdx.x >> 6;
-    const int64_t tiles = (dim + 63) / 64, work = joins[0] * tiles;
-    for (int64_t job = blockIdx.x; job < work; job += gridDim.x) {
-        const int64_t c = joins[1 + job / tiles], at = job % tiles * 64 + col;
-        const uint32_t key = keys[(c + 1) * span];
-        int64_t a = (c + 1) * span, b = n;                              // first place behind the id
-        while (a < b) {
-            const int64_t m = (a + b) >> 1;
-            if (keys[m] > key) b = m; else a = m + 1;
-        }
-        const int64_t last = (a - 1) / span;
-        float sum = 0.0f;
-        if (at < dim) {
-            if (s == 0) sum = partial[(c * 2 + 1) * dim + at];
-#pragma unroll 8
-            for (int64_t k = c + 1 + s; k <= last; k += 4) sum += partial[k * 2 * dim + at];
-        }
-        part[s][col] = sum;
+                                                             const uint32_t *__restrict__ goes_on, T *__restrict__ g_table) {
+    __shared__ float part[4][256];
+    const int64_t c = blockIdx.x, spans = (n + span - 1) / span;
+    if (!goes_on[c]) return;
+    const int lane = threadIdx.x & 63, s = threadIdx.x >> 6;
+    const uint32_t key = keys[(c + 1) * span];
+    // the last span that begins inside of the id: 64 spans a step, the steps growing by 64 while all of them do
+    int64_t last = c + 1, step = 1;
+    for (bool grow = true; step > 0;) {
+        const int64_t probe = last + (lane + 1) * step;
+        const uint64_t in = __ballot(probe < spans && keys[probe * span] == key);
+        const int more = in == ~0ull ? 64 : __ffsll((long long)~in) - 1;
+        last += more * step;
+        if (more < 64) grow = false;
+        step = grow ? step * 64 : step / 64;
+    }
+    for (int64_t base = (int64_t)blockIdx.y * 256; base < dim; base += (int64_t)gridDim.y * 256) {
+        const int64_t at = base + lane * 4;
+        float sum[4] = {};
+        auto add = [&](const float *row) {
+            const Row<float> r = nerf::load_flat(row + at, dim - at);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) sum[j] += r.v[j];
+        };
+        if (s == 0) add(partial + (c * 2 + 1) * dim);
+#pragma unroll 4
+        for (int64_t k = c + 1 + s; k <= last; k += 4) add(partial + k * 2 * dim);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) part[s][lane * 4 + j] = sum[j];
         __syncthreads();
-        if (s == 0 && at < dim)
-            g_table[(int64_t)key * dim + at] = (T)((part[0][col] + part[1][col] + part[2][col] + part[3][col]) * scale);
+        const int64_t col = base + threadIdx.x;
+        if (col < dim)
+            g_table[(int64_t)key * dim + col] = (T)((part[0][threadIdx.x] + part[1][threadIdx.x] + part[2][threadIdx.x] +
+                                                     part[3][threadIdx.x]) * scale);
         __syncthreads();
     }
 }
@@ -436,7 +463,7 @@ struct Plan {
     int64_t column_tiles;
     int chunk;                         // sorted pairs per lane group
     int64_t spans;                     // workgroups of the sum, along the pairs
-    int64_t keys, order, keys2, order2, counts, totals, partial, joins, bytes;   // offsets in the workspace
+    int64_t keys, order, keys2, order2, counts, totals, partial, goes_on, bytes;   // offsets in the workspace
 };
 
 int lane_shift(int64_t pieces) {
@@ -444,6 +471,10 @@ int lane_shift(int64_t pieces) {
     while (s < 8 && (1 << s) < pieces) ++s;
     return s;
 }
+
+// Of the sum: at least 8 lanes a row, or the chunks of a workgroup, added one after another, become too many (dim 1, 16384
+// pairs: 256 chunks took 37 us).
+constexpr int MIN_SUM_SHIFT = 3;
 
 Plan plan_backward(int64_t n, int64_t rows, int64_t dim, int dtype) {
     Plan p;
@@ -453,7 +484,7 @@ Plan plan_backward(int64_t n, int64_t rows, int64_t dim, int dtype) {
     p.bits = (bits + p.passes - 1) / p.passes;
     p.tiles = n <= ONE_TILE ? 0 : (n + TILE - 1) / TILE;
     const int64_t pieces = (dim * nerf::dtype_bytes(dtype) + 15) / 16;
-    p.shift = lane_shift(pieces);
+    p.shift = lane_shift(pieces) > MIN_SUM_SHIFT ? lane_shift(pieces) : MIN_SUM_SHIFT;
     p.column_tiles = (pieces + (1 << p.shift) - 1) >> p.shift;
     // about 8 wavefronts per SIMD of the chip, in lane groups; never fewer than 8 pairs a group
     const int64_t groups = ((int64_t)256 * 32 * WAVE >> p.shift) / p.column_tiles;
@@ -472,7 +503,7 @@ Plan plan_backward(int64_t n, int64_t rows, int64_t dim, int dtype) {
     p.counts = take(p.tiles ? 4 * (p.tiles << p.bits) : 0);
     p.totals = take(p.tiles ? 4 << p.bits : 0);
     p.partial = take(p.spans * 2 * dim * 4);
-    p.joins = take(4 * (1 + p.spans));
+    p.goes_on = take(4 * p.spans);
     p.bytes = at;
     return p;
 }
@@ -490,14 +521,14 @@ void launch_forward(const void *table, int64_t rows, int64_t row_stride, int64_t
     int64_t gx = (n + per - 1) / per, gy = (pieces + (1 << shift) - 1) >> shift;
     if (gx > 256 * 16) gx = 256 * 16;
     if (gy > 64) gy = 64;
-    hipLaunchKernelGGL(embedding_kernel<T>, dim3((unsigned)gx, (unsigned)gy), dim3(256), 0, stream,
-                       static_cast<const T *>(table), rows, row_stride, dim, ids, wide, n, scale, shift,
-                       static_cast<T *>(out));
+    auto kernel = dim < Row<T>::VEC ? embedding_kernel<T, true> : embedding_kernel<T, false>;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)gx, (unsigned)gy), dim3(256), 0, stream, static_cast<const T *>(table), rows,
+                       row_stride, (int)dim, ids, wide, n, scale, shift, static_cast<T *>(out));
 }
 
 template <typename T, int ITEMS>
-int launch_sort_one(const Plan &p, int64_t clear_blocks, const void *ids, int wide, int64_t n, int64_t rows,
-                    int64_t padding_idx, uint32_t *keys, uint32_t *order, uint32_t *joins, T *g_table, int64_t count,
+int launch_sort_one(const Plan &p, int64_t clear_blocks, int64_t per, const void *ids, int wide, int64_t n, int64_t rows,
+                    int64_t padding_idx, uint32_t *keys, uint32_t *order, T *g_table, int64_t count,
                     hipStream_t stream) {
     static nerf::DeviceMask done;
     auto kernel = embedding_sort_one_kernel<T, ITEMS>;
@@ -505,7 +536,7 @@ int launch_sort_one(const Plan &p, int64_t clear_blocks, const void *ids, int wi
                                           "nerf_embedding_backward"))
         return rc;
     hipLaunchKernelGGL(kernel, dim3((unsigned)(1 + clear_blocks)), dim3(SORT_THREADS), one_lds_bytes<ITEMS>(p.bits), stream,
-                       ids, wide, (int)n, rows, padding_idx, p.passes, p.bits, keys, order, joins, g_table, count);
+                       ids, wide, (int)n, rows, padding_idx, p.passes, p.bits, keys, order, g_table, count, per);
     return NERF_OK;
 }
 
@@ -513,22 +544,23 @@ template <typename T>
 int launch_backward(const void *g_out, int dtype, int64_t n, int64_t dim, const void *ids, int wide, int64_t rows, float scale,
                     int64_t padding_idx, void *g_table, char *ws, hipStream_t stream) {
     T *gt = static_cast<T *>(g_table);
-    const int64_t count = rows * dim, per_block = (int64_t)SORT_THREADS * Row<T>::VEC;
-    int64_t clear_blocks = (count + per_block - 1) / per_block;
+    const int64_t count = rows * dim, pieces = (count + Row<T>::VEC - 1) / Row<T>::VEC;
+    int64_t clear_blocks = (pieces + SORT_THREADS - 1) / SORT_THREADS;
     if (clear_blocks > 1024) clear_blocks = 1024;
+    const int64_t per = (pieces + clear_blocks - 1) / clear_blocks;
     if (n == 0) {
-        hipLaunchKernelGGL(embedding_zero_kernel<T>, dim3((unsigned)clear_blocks), dim3(SORT_THREADS), 0, stream, gt, count);
+        hipLaunchKernelGGL(embedding_zero_kernel<T>, dim3((unsigned)clear_blocks), dim3(SORT_THREADS), 0, stream, gt, count, per);
         return NERF_OK;
     }
     const Plan p = plan_backward(n, rows, dim, dtype);
     auto words = [&](int64_t offset) { return reinterpret_cast<uint32_t *>(ws + offset); };
-    uint32_t *keys = words(p.keys), *order = words(p.order), *joins = words(p.joins);
+    uint32_t *keys = words(p.keys), *order = words(p.order);
     float *partial = reinterpret_cast<float *>(ws + p.partial);
     if (!p.tiles) {
         auto sort = n <= SORT_THREADS       ? launch_sort_one<T, 1>
                     : n <= SORT_THREADS * 4 ? launch_sort_one<T, 4>
                                             : launch_sort_one<T, 16>;
-        if (int rc = sort(p, clear_blocks, ids, wide, n, rows, padding_idx, keys, order, joins, gt, count, stream)) return rc;
+        if (int rc = sort(p, clear_blocks, per, ids, wide, n, rows, padding_idx, keys, order, gt, count, stream)) return rc;
     } else {
         // the last pass has to end in `keys`
         uint32_t *k[2] = {keys, words(p.keys2)}, *o[2] = {order, words(p.order2)};
@@ -537,20 +569,22 @@ int launch_backward(const void *g_out, int dtype, int64_t n, int64_t dim, const 
             const uint32_t *ki = q ? k[to ^ 1] : nullptr, *oi = q ? o[to ^ 1] : nullptr;
             hipLaunchKernelGGL(embedding_sort_count_kernel<T>, dim3((unsigned)(p.tiles + (q ? 0 : clear_blocks))),
                                dim3(SORT_THREADS), 0, stream, ids, wide, n, rows, padding_idx, ki, q * p.bits, p.bits, p.tiles,
-                               words(p.counts), joins, gt, count);
+                               words(p.counts), gt, count, per);
             hipLaunchKernelGGL(embedding_sort_scan_kernel, dim3(1u << p.bits), dim3(SORT_THREADS), 0, stream, words(p.counts),
                                p.tiles, words(p.totals));
             hipLaunchKernelGGL(embedding_sort_move_kernel, dim3((unsigned)p.tiles), dim3(SORT_THREADS), 0, stream, ids, wide,
                                n, rows, padding_idx, ki, oi, q * p.bits, p.bits, words(p.totals), words(p.counts), k[to], o[to]);
         }
     }
-    hipLaunchKernelGGL(embedding_sum_kernel<T>, dim3((unsigned)p.spans, (unsigned)p.column_tiles), dim3(SUM_THREADS), 0, stream,
-                       static_cast<const T *>(g_out), n, dim, keys, order, (uint32_t)rows, scale, p.chunk, p.shift, gt, partial,
-                       joins);
+    auto sum = dim < Row<T>::VEC ? embedding_sum_kernel<T, true> : embedding_sum_kernel<T, false>;
+    hipLaunchKernelGGL(sum, dim3((unsigned)p.spans, (unsigned)p.column_tiles), dim3(SUM_THREADS), 0, stream,
+                       static_cast<const T *>(g_out), n, (int)dim, keys, order, (uint32_t)rows, scale, p.chunk, p.shift, gt, partial,
+                       words(p.goes_on));
     if (p.spans > 1) {
-        const int64_t most = (p.spans - 1) * ((dim + 63) / 64);
-        hipLaunchKernelGGL(embedding_join_kernel<T>, dim3((unsigned)(most < 1024 ? most : 1024)), dim3(256), 0, stream, keys, n,
-                           dim, scale, (int64_t)p.chunk * (SUM_THREADS >> p.shift), partial, joins, gt);
+        int64_t gy = (dim + 255) / 256;
+        hipLaunchKernelGGL(embedding_join_kernel<T>, dim3((unsigned)(p.spans - 1), (unsigned)(gy < 16 ? gy : 16)), dim3(256), 0,
+                           stream, keys, n, dim, scale, (int64_t)p.chunk * (SUM_THREADS >> p.shift), partial,
+                           words(p.goes_on), gt);
     }
     return NERF_OK;
 }

@@ -1,8 +1,10 @@
 // Rows of fp32 / bf16 / fp16 values for the learned-code operators (layernorm.hip, dropout.hip, embedding.hip).
 //
 // A row is moved in 16-byte pieces per lane whatever its address: gfx950 serves a global dwordx4 access at any element
-// boundary, so an odd row length needs no variant of its own.  Only the piece that a row ends in goes value by value:
-// nothing is read or written beyond a row.  Arithmetic is fp32; a value is rounded once, when it is stored.
+// boundary, so an odd row length needs no variant of its own.  The piece that a row ends in is moved back to end with the
+// row: it holds some values of its neighbour again (`Place::own` tells them apart), so that no access goes value by value
+// and none leaves the row.  Only rows shorter than a piece (TINY) do.  Arithmetic is fp32; a value is rounded once, when
+// it is stored.
 #pragma once
 #include "common.h"
 
@@ -14,9 +16,68 @@ struct Row {
     T v[VEC];
 };
 
-// `count` values (any number; <= 0: none) starting at p; missing ones read as 0
+// Where the piece that would begin at value `a` of a row of C values is: at `at`, with its first `skip` values another's.
+// skip >= VEC: the row ends before it.
+template <typename T, bool TINY>
+struct Place {
+    int at, skip, C;
+    __device__ __forceinline__ Place(int a, int C_) : at(TINY ? a : (a < C_ - Row<T>::VEC ? a : C_ - Row<T>::VEC)), skip(a - at), C(C_) {}
+    __device__ __forceinline__ bool live() const { return TINY ? at < C : skip < Row<T>::VEC; }
+    // unsigned: a uniform row pointer then stays in scalar registers, with 32 bits per lane beside it
+    __device__ __forceinline__ uint32_t bytes() const { return (uint32_t)at * (uint32_t)sizeof(T); }
+    __device__ __forceinline__ bool own(int j) const { return TINY ? at + j < C : j >= skip; }
+};
+
+template <bool TINY, typename T>
+__device__ __forceinline__ Row<T> load_piece(const T *row, const Place<T, TINY> &p) {
+    Row<T> r;
+    if (TINY) {
+#pragma unroll
+        for (int j = 0; j < Row<T>::VEC; ++j) r.v[j] = p.own(j) ? row[p.at + j] : (T)0.0f;
+    } else {
+        __builtin_memcpy(&r, reinterpret_cast<const char *>(row) + p.bytes(), 16);
+    }
+    return r;
+}
+
+// (values shared with the neighbouring piece are stored twice, the same)
+template <bool TINY, typename T>
+__device__ __forceinline__ void store_piece(T *row, const Place<T, TINY> &p, const Row<T> &r) {
+    if (TINY) {
+#pragma unroll
+        for (int j = 0; j < Row<T>::VEC; ++j)
+            if (p.own(j)) row[p.at + j] = r.v[j];
+    } else if (p.live()) {
+        __builtin_memcpy(reinterpret_cast<char *>(row) + p.bytes(), &r, 16);
+    }
+}
+
+// the same piece of the weights, as fp32: of the row's own type, or fp32; `absent` where there are none
+template <bool TINY, typename T>
+__device__ __forceinline__ void load_weights(const void *w, bool w_f32, const Place<T, TINY> &p, float absent,
+                                             float (&out)[Row<T>::VEC]) {
+    constexpr int VEC = Row<T>::VEC;
+    if (w == nullptr) {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) out[j] = absent;
+    } else if (sizeof(T) == 2 && w_f32) {
+        const float *f = reinterpret_cast<const float *>(static_cast<const char *>(w) + (uint32_t)p.at * 4u);
+        if (TINY) {
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) out[j] = p.own(j) ? f[j] : 0.0f;
+        } else {
+            __builtin_memcpy(out, f, VEC * 4);
+        }
+    } else {
+        const Row<T> r = load_piece<TINY>(static_cast<const T *>(w), p);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) out[j] = (float)r.v[j];
+    }
+}
+
+// The end of a flat array: `count` values starting at p, fewer than a piece only at its end.
 template <typename T>
-__device__ __forceinline__ Row<T> load_piece(const T *p, int64_t count) {
+__device__ __forceinline__ Row<T> load_flat(const T *p, int64_t count) {
     Row<T> r;
     if (count >= Row<T>::VEC) {
         __builtin_memcpy(&r, p, 16);
@@ -28,7 +89,7 @@ __device__ __forceinline__ Row<T> load_piece(const T *p, int64_t count) {
 }
 
 template <typename T>
-__device__ __forceinline__ void store_piece(T *p, const Row<T> &r, int64_t count) {
+__device__ __forceinline__ void store_flat(T *p, const Row<T> &r, int64_t count) {
     if (count >= Row<T>::VEC) {
         __builtin_memcpy(p, &r, 16);
     } else {
@@ -38,27 +99,11 @@ __device__ __forceinline__ void store_piece(T *p, const Row<T> &r, int64_t count
     }
 }
 
-// VEC consecutive weights as fp32: of the row's own type, or fp32
-template <typename T>
-__device__ __forceinline__ void load_weights(const void *w, bool w_f32, int64_t at, int64_t count, float absent,
-                                             float (&out)[Row<T>::VEC]) {
-    constexpr int VEC = Row<T>::VEC;
-    if (w == nullptr) {
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) out[j] = absent;
-    } else if (sizeof(T) == 2 && w_f32) {
-        const float *p = static_cast<const float *>(w) + at;
-#pragma unroll
-        for (int h = 0; h < VEC; h += 4) {
-            const Row<float> r = load_piece(p + h, count - h);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) out[h + j] = r.v[j];
-        }
-    } else {
-        const Row<T> r = load_piece(static_cast<const T *>(w) + at, count);
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) out[j] = (float)r.v[j];
-    }
+// Which group of TPR threads this thread is in; a scalar where a wavefront is in one group.
+template <int TPR>
+__device__ __forceinline__ int lane_group() {
+    const int g = threadIdx.x / TPR;
+    return TPR >= WAVE ? __builtin_amdgcn_readfirstlane(g) : g;
 }
 
 // sum over groups of WIDTH lanes (a power of two <= 64), every lane gets it
