@@ -16,56 +16,79 @@ using nerf::Row;
 
 constexpr uint64_t GAMMA = 0xD1342543DE82EF95ull;
 
-__device__ __forceinline__ uint64_t mix(uint64_t x) {
-    x = (x ^ (x >> 30)) * 0xBF58476D1CE4E5B9ull;
-    x = (x ^ (x >> 27)) * 0x94D049BB133111EBull;
-    return x ^ (x >> 31);
+// The finaliser on 32-bit halves: its 64-bit shifts as an align and a shift, which run at full rate.
+struct Word {
+    uint32_t lo, hi;
+};
+
+template <int SHIFT>
+__device__ __forceinline__ Word fold(Word x) {               // x ^ (x >> SHIFT)
+    return {x.lo ^ __builtin_amdgcn_alignbit(x.hi, x.lo, SHIFT), x.hi ^ (x.hi >> SHIFT)};
 }
 
-// ODD: the global index of element 0 is odd, so that every pair of elements takes halves of two words
+__device__ __forceinline__ Word times(Word x, uint64_t c) {
+    const uint64_t low = (uint64_t)x.lo * (uint32_t)c;
+    return {(uint32_t)low, (uint32_t)(low >> 32) + x.lo * (uint32_t)(c >> 32) + x.hi * (uint32_t)c};
+}
+
+__device__ __forceinline__ Word mix(uint64_t state) {
+    Word x = {(uint32_t)state, (uint32_t)(state >> 32)};
+    x = times(fold<30>(x), 0xBF58476D1CE4E5B9ull);
+    x = times(fold<27>(x), 0x94D049BB133111EBull);
+    return fold<31>(x);
+}
+
+// A piece a thread.  ODD: the global index of element 0 is odd, so that every pair of elements takes halves of two words.
 template <typename T, bool ODD, bool ADD>
 __global__ __launch_bounds__(256) void dropout_kernel(const T *__restrict__ x, const T *__restrict__ residual, int64_t n,
-                                                      uint64_t threshold, float scale, uint64_t key,
+                                                      uint32_t threshold, bool none, float scale, uint64_t key,
                                                       const uint64_t *__restrict__ key_dev, int64_t first,
                                                       T *__restrict__ out) {
     constexpr int VEC = Row<T>::VEC, WORDS = VEC / 2 + (ODD ? 1 : 0);
     if (key_dev) key = *key_dev;
-    const int64_t pieces = (n + VEC - 1) / VEC;
-    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < pieces; i += (int64_t)gridDim.x * blockDim.x) {
-        const int64_t at = i * VEC, count = n - at;
-        const Row<T> a = nerf::load_flat(x + at, count);
+    const int64_t pieces = n / VEC, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i < pieces) {
+        const int64_t at = i * VEC;
+        const Row<T> a = nerf::load_16<T>(x + at);
         Row<T> r;
-        if (ADD) r = nerf::load_flat(residual + at, count);
-        uint64_t state = key + (uint64_t)((first + at) >> 1) * GAMMA;
+        if (ADD) r = nerf::load_16<T>(residual + at);
+        // (first + at) / 2 in a part that is the workgroup's and one that is the thread's: a multiplication less a thread
+        uint64_t state = key + ((uint64_t)(first >> 1) + (uint64_t)blockIdx.x * (256 * VEC / 2)) * GAMMA +
+                         (uint64_t)(threadIdx.x * (VEC / 2)) * GAMMA;
         uint32_t bits[2 * WORDS];
 #pragma unroll
         for (int j = 0; j < WORDS; ++j) {
-            const uint64_t w = mix(state);
-            bits[2 * j] = (uint32_t)w;
-            bits[2 * j + 1] = (uint32_t)(w >> 32);
+            const Word w = mix(state);
+            bits[2 * j] = w.lo;
+            bits[2 * j + 1] = w.hi;
             state += GAMMA;
         }
         Row<T> y;
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
-            const bool keep = bits[j + (ODD ? 1 : 0)] >= threshold;
-            const float v = keep ? (float)a.v[j] * scale : 0.0f;
+            const float v = bits[j + (ODD ? 1 : 0)] >= threshold && !none ? (float)a.v[j] * scale : 0.0f;
             y.v[j] = (T)(ADD ? (float)r.v[j] + v : v);
         }
-        nerf::store_flat(out + at, y, count);
+        nerf::store_16(out + at, y);
+    }
+    // what is left behind the last whole piece
+    const int64_t at = pieces * VEC + threadIdx.x;
+    if (blockIdx.x == 0 && at < n) {
+        const Word w = mix(key + (uint64_t)((first + at) >> 1) * GAMMA);
+        const float v = (((first + at) & 1) ? w.hi : w.lo) >= threshold && !none ? (float)x[at] * scale : 0.0f;
+        out[at] = (T)(ADD ? (float)residual[at] + v : v);
     }
 }
 
 template <typename T>
-void launch(const void *x, const void *residual, int64_t n, uint64_t threshold, float scale, uint64_t key,
+void launch(const void *x, const void *residual, int64_t n, uint32_t threshold, bool none, float scale, uint64_t key,
             const uint64_t *key_dev, int64_t first, void *out, hipStream_t stream) {
     const int64_t pieces = (n + Row<T>::VEC - 1) / Row<T>::VEC;
-    int64_t grid = (pieces + 255) / 256;
-    if (grid > 256 * 16) grid = 256 * 16;
+    const int64_t grid = (pieces + 255) / 256;
     auto kernel = residual ? ((first & 1) ? dropout_kernel<T, true, true> : dropout_kernel<T, false, true>)
                            : ((first & 1) ? dropout_kernel<T, true, false> : dropout_kernel<T, false, false>);
     hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(256), 0, stream, static_cast<const T *>(x),
-                       static_cast<const T *>(residual), n, threshold, scale, key, key_dev, first, static_cast<T *>(out));
+                       static_cast<const T *>(residual), n, threshold, none, scale, key, key_dev, first, static_cast<T *>(out));
 }
 
 }  // namespace
@@ -73,12 +96,13 @@ void launch(const void *x, const void *residual, int64_t n, uint64_t threshold, 
 NERF_API int nerf_dropout(const void *x, const void *residual, int dtype, int64_t n, double p, uint64_t key,
                           const uint64_t *key_dev, int64_t first, void *out, nerf_stream_t stream) {
     NERF_REQUIRE(nerf::known_dtype(dtype), "nerf_dropout: unknown dtype");
-    NERF_REQUIRE(n >= 0 && first >= 0 && first <= INT64_MAX - n, "nerf_dropout: element range out of bounds");
+    NERF_REQUIRE(n >= 0 && n <= (int64_t)1 << 40 && first >= 0 && first <= INT64_MAX - n, "nerf_dropout: element range out of bounds");
     NERF_REQUIRE(p >= 0.0 && p <= 1.0, "nerf_dropout: p must be in [0, 1]");
     if (n == 0) return NERF_OK;
     NERF_REQUIRE(x && out, "nerf_dropout: null pointer");
     const uint64_t threshold = (uint64_t)floor(p * 4294967296.0 + 0.5);      // 2^32 (p = 1): nothing is kept
     const float scale = p < 1.0 ? (float)(1.0 / (1.0 - p)) : 0.0f;
-    NERF_FOR_DTYPE(dtype, T, launch<T>(x, residual, n, threshold, scale, key, key_dev, first, out, nerf::as_stream(stream)));
+    NERF_FOR_DTYPE(dtype, T, launch<T>(x, residual, n, (uint32_t)threshold, threshold >> 32, scale, key, key_dev, first, out,
+                                       nerf::as_stream(stream)));
     return nerf::check_launch("nerf_dropout");
 }

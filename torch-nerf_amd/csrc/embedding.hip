@@ -50,11 +50,9 @@ __device__ __forceinline__ void clear(T *g_table, int64_t count, int64_t per, in
     Row<T> zero;
 #pragma unroll
     for (int j = 0; j < Row<T>::VEC; ++j) zero.v[j] = (T)0.0f;
-    const int64_t hi = (block + 1) * per;
-    for (int64_t i = block * per + threadIdx.x; i < hi; i += blockDim.x) {
-        const int64_t at = i * Row<T>::VEC;
-        if (at < count) nerf::store_flat(g_table + at, zero, count - at);
-    }
+    const int64_t whole = count / Row<T>::VEC, hi = (block + 1) * per < whole ? (block + 1) * per : whole;
+    for (int64_t i = block * per + threadIdx.x; i < hi; i += blockDim.x) nerf::store_16(g_table + i * Row<T>::VEC, zero);
+    if (block == 0 && (int)threadIdx.x < (int)(count - whole * Row<T>::VEC)) g_table[whole * Row<T>::VEC + threadIdx.x] = zero.v[0];
 }
 
 template <typename T>
@@ -414,8 +412,8 @@ __global__ __launch_bounds__(SUM_THREADS) void embedding_sum_kernel(const T *__r
 
 // One workgroup a span and 256 columns, 4 a lane; it has work where an id begins in the span and goes on behind it: the
 // first partial row and those of the spans that follow, one wavefront every fourth of them.
-template <typename T>
-__global__ __launch_bounds__(256) void embedding_join_kernel(const uint32_t *__restrict__ keys, int64_t n, int64_t dim,
+template <typename T, bool TINY>
+__global__ __launch_bounds__(256) void embedding_join_kernel(const uint32_t *__restrict__ keys, int64_t n, int dim,
                                                              float scale, int64_t span, const float *__restrict__ partial,
                                                              const uint32_t *__restrict__ goes_on, T *__restrict__ g_table) {
     __shared__ float part[4][256];
@@ -433,24 +431,24 @@ __global__ __launch_bounds__(256) void embedding_join_kernel(const uint32_t *__r
         if (more < 64) grow = false;
         step = grow ? step * 64 : step / 64;
     }
-    for (int64_t base = (int64_t)blockIdx.y * 256; base < dim; base += (int64_t)gridDim.y * 256) {
-        const int64_t at = base + lane * 4;
+    for (int base = blockIdx.y * 256; base < dim; base += gridDim.y * 256) {
+        const nerf::Place<float, TINY> at(base + lane * 4, dim);
         float sum[4] = {};
-        auto add = [&](const float *row) {
-            const Row<float> r = nerf::load_flat(row + at, dim - at);
+        auto add = [&](int64_t k, int which) {
+            const Row<float> r = nerf::load_piece<TINY>(partial + (k * 2 + which) * dim, at);
 #pragma unroll
             for (int j = 0; j < 4; ++j) sum[j] += r.v[j];
         };
-        if (s == 0) add(partial + (c * 2 + 1) * dim);
+        if (s == 0) add(c, 1);
 #pragma unroll 4
-        for (int64_t k = c + 1 + s; k <= last; k += 4) add(partial + k * 2 * dim);
+        for (int64_t k = c + 1 + s; k <= last; k += 4) add(k, 0);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) part[s][lane * 4 + j] = sum[j];
+        for (int j = 0; j < 4; ++j)
+            if (at.own(j)) part[s][at.at + j - base] = sum[j];
         __syncthreads();
-        const int64_t col = base + threadIdx.x;
-        if (col < dim)
-            g_table[(int64_t)key * dim + col] = (T)((part[0][threadIdx.x] + part[1][threadIdx.x] + part[2][threadIdx.x] +
-                                                     part[3][threadIdx.x]) * scale);
+        const int col = threadIdx.x;
+        if (base + col < dim)
+            g_table[(int64_t)key * dim + base + col] = (T)((part[0][col] + part[1][col] + part[2][col] + part[3][col]) * scale);
         __syncthreads();
     }
 }
@@ -582,9 +580,9 @@ int launch_backward(const void *g_out, int dtype, int64_t n, int64_t dim, const 
                        words(p.goes_on));
     if (p.spans > 1) {
         int64_t gy = (dim + 255) / 256;
-        hipLaunchKernelGGL(embedding_join_kernel<T>, dim3((unsigned)(p.spans - 1), (unsigned)(gy < 16 ? gy : 16)), dim3(256), 0,
-                           stream, keys, n, dim, scale, (int64_t)p.chunk * (SUM_THREADS >> p.shift), partial,
-                           words(p.goes_on), gt);
+        auto join = dim < Row<float>::VEC ? embedding_join_kernel<T, true> : embedding_join_kernel<T, false>;
+        hipLaunchKernelGGL(join, dim3((unsigned)(p.spans - 1), (unsigned)(gy < 16 ? gy : 16)), dim3(256), 0, stream, keys, n,
+                           (int)dim, scale, (int64_t)p.chunk * (SUM_THREADS >> p.shift), partial, words(p.goes_on), gt);
     }
     return NERF_OK;
 }

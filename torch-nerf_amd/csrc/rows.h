@@ -16,6 +16,21 @@ struct Row {
     T v[VEC];
 };
 
+// One 16-byte access at an element's alignment.  As a vector of words: a copy value by value is taken apart by the compiler
+// where only some values are used on some path.
+typedef uint32_t words __attribute__((ext_vector_type(4)));
+typedef words loose_words __attribute__((aligned(2)));
+
+template <typename T>
+__device__ __forceinline__ Row<T> load_16(const void *p) {
+    return __builtin_bit_cast(Row<T>, static_cast<words>(*static_cast<const loose_words *>(p)));
+}
+
+template <typename T>
+__device__ __forceinline__ void store_16(void *p, const Row<T> &r) {
+    *static_cast<loose_words *>(p) = __builtin_bit_cast(words, r);
+}
+
 // Where the piece that would begin at value `a` of a row of C values is: at `at`, with its first `skip` values another's.
 // skip >= VEC: the row ends before it.
 template <typename T, bool TINY>
@@ -35,7 +50,7 @@ __device__ __forceinline__ Row<T> load_piece(const T *row, const Place<T, TINY> 
 #pragma unroll
         for (int j = 0; j < Row<T>::VEC; ++j) r.v[j] = p.own(j) ? row[p.at + j] : (T)0.0f;
     } else {
-        __builtin_memcpy(&r, reinterpret_cast<const char *>(row) + p.bytes(), 16);
+        r = load_16<T>(reinterpret_cast<const char *>(row) + p.bytes());
     }
     return r;
 }
@@ -48,7 +63,7 @@ __device__ __forceinline__ void store_piece(T *row, const Place<T, TINY> &p, con
         for (int j = 0; j < Row<T>::VEC; ++j)
             if (p.own(j)) row[p.at + j] = r.v[j];
     } else if (p.live()) {
-        __builtin_memcpy(reinterpret_cast<char *>(row) + p.bytes(), &r, 16);
+        store_16(reinterpret_cast<char *>(row) + p.bytes(), r);
     }
 }
 
@@ -72,30 +87,6 @@ __device__ __forceinline__ void load_weights(const void *w, bool w_f32, const Pl
         const Row<T> r = load_piece<TINY>(static_cast<const T *>(w), p);
 #pragma unroll
         for (int j = 0; j < VEC; ++j) out[j] = (float)r.v[j];
-    }
-}
-
-// The end of a flat array: `count` values starting at p, fewer than a piece only at its end.
-template <typename T>
-__device__ __forceinline__ Row<T> load_flat(const T *p, int64_t count) {
-    Row<T> r;
-    if (count >= Row<T>::VEC) {
-        __builtin_memcpy(&r, p, 16);
-    } else {
-#pragma unroll
-        for (int j = 0; j < Row<T>::VEC; ++j) r.v[j] = j < count ? p[j] : (T)0.0f;
-    }
-    return r;
-}
-
-template <typename T>
-__device__ __forceinline__ void store_flat(T *p, const Row<T> &r, int64_t count) {
-    if (count >= Row<T>::VEC) {
-        __builtin_memcpy(p, &r, 16);
-    } else {
-#pragma unroll
-        for (int j = 0; j < Row<T>::VEC; ++j)
-            if (j < count) p[j] = r.v[j];
     }
 }
 
