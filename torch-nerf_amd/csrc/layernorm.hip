@@ -8,38 +8,54 @@
 // sums are fp32.  Rows of up to 64 lanes need no barrier; a longer row takes a workgroup.
 #include "rows.h"
 
-#ifndef X_AHEAD
-#define X_AHEAD 0
-#endif
 namespace {
 
 using nerf::Row;
 
-// Sum of K values over the TPR lanes that share a row.  TPR > 64: through LDS, every group of TPR threads of the workgroup
-// at once; `slot` alternates so that one barrier per sum is enough (a wave that runs ahead writes the other half of `red`).
-template <int TPR, int K, int BLOCK>
-__device__ __forceinline__ void row_sum(float (&v)[K], float *red, int &slot) {
+// Rows of at most one wavefront's registers: TPR <= 64 lanes share one.  Wider rows take `waves` wavefronts each (WIDE), as
+// many as the row needs, and a workgroup a whole number of such groups.
+//
+// Sum of K values over the lanes that share a row.  WIDE: through LDS, all groups of the workgroup at once; `slot`
+// alternates so that one barrier per sum is enough (a wave that runs ahead writes the other half of `red`).
+constexpr int MAX_WAVES = 16;
+
+template <int TPR, bool WIDE, int K>
+__device__ __forceinline__ void row_sum(float (&v)[K], float *red, int &slot, int waves) {
 #pragma unroll
-    for (int k = 0; k < K; ++k) v[k] = nerf::lane_sum<(TPR < WAVE ? TPR : WAVE)>(v[k]);
-    if constexpr (TPR > WAVE) {
-        constexpr int WAVES = TPR / WAVE;
-        float *r = red + slot * (BLOCK / WAVE) * K;
+    for (int k = 0; k < K; ++k) v[k] = nerf::lane_sum<TPR>(v[k]);
+    if constexpr (WIDE) {
+        const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
+        float *r = red + slot * MAX_WAVES * K;
         slot ^= 1;
         if ((threadIdx.x & (WAVE - 1)) == 0) {
 #pragma unroll
-            for (int k = 0; k < K; ++k) r[(threadIdx.x / WAVE) * K + k] = v[k];
+            for (int k = 0; k < K; ++k) r[wave * K + k] = v[k];
         }
         __syncthreads();
-        r += threadIdx.x / TPR * WAVES * K;
+        const int w = threadIdx.x & (MAX_WAVES - 1);
+        r += (wave / waves * waves + (w < waves ? w : 0)) * K;
 #pragma unroll
-        for (int k = 0; k < K; ++k) {
-            float s = 0.0f;
-#pragma unroll
-            for (int w = 0; w < WAVES; ++w) s += r[w * K + k];
-            v[k] = s;
-        }
+        for (int k = 0; k < K; ++k) v[k] = nerf::lane_sum<MAX_WAVES>(w < waves ? r[k] : 0.0f);
     }
 }
+
+// Which of its row's lanes a thread is, and which row of its workgroup's (a scalar where a wavefront has one row).
+template <int TPR, bool WIDE>
+struct Lanes {
+    int lane, group, width;
+    __device__ __forceinline__ explicit Lanes(int waves) {
+        const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
+        if (WIDE) {
+            group = wave / waves;
+            lane = (int)threadIdx.x - group * waves * WAVE;
+            width = waves * WAVE;
+        } else {
+            group = TPR == WAVE ? wave : (int)threadIdx.x / TPR;
+            lane = threadIdx.x % TPR;
+            width = TPR;
+        }
+    }
+};
 
 // The compiler may not keep what it made of p (or loaded through p) before this point.
 template <typename T>
@@ -50,45 +66,50 @@ __device__ __forceinline__ void forget(Row<T> &p) {
     __builtin_memcpy(&p, u, 16);
 }
 
-template <typename T, int TPR, int NV, int BLOCK, bool TINY>
-__global__ __launch_bounds__(BLOCK) void layernorm_kernel(const T *__restrict__ x, int64_t x_stride, int64_t M, int C,
+template <typename T, int TPR, int NV, bool WIDE, bool TINY>
+__global__ __launch_bounds__(WIDE ? 1024 : 256) void layernorm_kernel(const T *__restrict__ x, int64_t x_stride, int64_t M, int C,
                                                           const void *__restrict__ weight, const void *__restrict__ bias,
                                                           int w_f32, float eps, T *__restrict__ y,
-                                                          float *__restrict__ mean, float *__restrict__ rstd) {
-    constexpr int VEC = Row<T>::VEC, RPB = BLOCK / TPR;
+                                                          float *__restrict__ mean, float *__restrict__ rstd, int waves, int per) {
+    constexpr int VEC = Row<T>::VEC;
     constexpr bool HOIST = NV * VEC <= 8;                     // the weights stay in registers from row to row
-    static_assert(TPR <= WAVE || TPR == BLOCK, "a row beyond one wavefront takes the whole workgroup");
-    __shared__ float red[TPR > WAVE ? 2 * (BLOCK / WAVE) : 1];
+    __shared__ float red[WIDE ? 2 * MAX_WAVES : 1];
     int slot = 0;
-    const int lane = threadIdx.x % TPR;
+    const Lanes<TPR, WIDE> at_row(waves);                     // (WIDE: one row a workgroup)
+    const int lane = at_row.lane, width = at_row.width;
+    const int64_t rows = WIDE ? 1 : 256 / TPR;
     const float inv_c = 1.0f / (float)C;
     float w[HOIST ? NV : 1][VEC], b[HOIST ? NV : 1][VEC];
     if constexpr (HOIST) {
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const nerf::Place<T, TINY> at((i * TPR + lane) * VEC, C);
+            const nerf::Place<T, TINY> at((i * width + lane) * VEC, C);
             nerf::load_weights<TINY, T>(weight, w_f32, at, 1.0f, w[i]);
             nerf::load_weights<TINY, T>(bias, w_f32, at, 0.0f, b[i]);
         }
     }
-    for (int64_t row = (int64_t)blockIdx.x * RPB + nerf::lane_group<TPR>(); row < M; row += (int64_t)gridDim.x * RPB) {
+    const int64_t begin = (int64_t)blockIdx.x * per * rows, end = begin + per * rows < M ? begin + per * rows : M;
+    for (int64_t row = begin + at_row.group; row < end; row += rows) {
         float v[NV][VEC], s[1] = {0.0f};
+        Row<T> p[NV];
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+            p[i] = nerf::load_piece<TINY>(x + row * x_stride, nerf::Place<T, TINY>((i * width + lane) * VEC, C));
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const nerf::Place<T, TINY> at((i * TPR + lane) * VEC, C);
-            const Row<T> p = nerf::load_piece<TINY>(x + row * x_stride, at);
+            const nerf::Place<T, TINY> at((i * width + lane) * VEC, C);
 #pragma unroll
             for (int j = 0; j < VEC; ++j) {
-                v[i][j] = (float)p.v[j];
+                v[i][j] = (float)p[i].v[j];
                 s[0] += at.own(j) ? v[i][j] : 0.0f;
             }
         }
-        row_sum<TPR, 1, BLOCK>(s, red, slot);
+        row_sum<TPR, WIDE, 1>(s, red, slot, waves);
         const float mu = s[0] * inv_c;
         s[0] = 0.0f;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const nerf::Place<T, TINY> at((i * TPR + lane) * VEC, C);
+            const nerf::Place<T, TINY> at((i * width + lane) * VEC, C);
 #pragma unroll
             for (int j = 0; j < VEC; ++j) {
                 v[i][j] -= mu;
@@ -96,7 +117,7 @@ __global__ __launch_bounds__(BLOCK) void layernorm_kernel(const T *__restrict__ 
                 s[0] = fmaf(d, d, s[0]);
             }
         }
-        row_sum<TPR, 1, BLOCK>(s, red, slot);
+        row_sum<TPR, WIDE, 1>(s, red, slot, waves);
         const float r = 1.0f / sqrtf(s[0] * inv_c + eps);
         if (lane == 0) {
             if (mean) mean[row] = mu;
@@ -104,7 +125,7 @@ __global__ __launch_bounds__(BLOCK) void layernorm_kernel(const T *__restrict__ 
         }
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const nerf::Place<T, TINY> at((i * TPR + lane) * VEC, C);
+            const nerf::Place<T, TINY> at((i * width + lane) * VEC, C);
             if constexpr (!HOIST) {
                 nerf::load_weights<TINY, T>(weight, w_f32, at, 1.0f, w[0]);
                 nerf::load_weights<TINY, T>(bias, w_f32, at, 0.0f, b[0]);
@@ -137,7 +158,7 @@ __global__ __launch_bounds__(1024) void layernorm_long_kernel(const T *__restric
 #pragma unroll
             for (int j = 0; j < VEC; ++j) s[0] += at.own(j) ? (float)p.v[j] : 0.0f;
         }
-        row_sum<1024, 1, 1024>(s, red, slot);
+        row_sum<WAVE, true, 1>(s, red, slot, MAX_WAVES);
         const float mu = s[0] * inv_c;
         s[0] = 0.0f;
         for (int a = threadIdx.x * VEC; a < C; a += 1024 * VEC) {
@@ -149,7 +170,7 @@ __global__ __launch_bounds__(1024) void layernorm_long_kernel(const T *__restric
                 s[0] = fmaf(d, d, s[0]);
             }
         }
-        row_sum<1024, 1, 1024>(s, red, slot);
+        row_sum<WAVE, true, 1>(s, red, slot, MAX_WAVES);
         const float r = 1.0f / sqrtf(s[0] * inv_c + eps);
         if (threadIdx.x == 0) {
             if (mean) mean[row] = mu;
@@ -175,25 +196,27 @@ __global__ __launch_bounds__(1024) void layernorm_long_kernel(const T *__restric
 // A row stays in registers as it was read; h and q are made from it twice (`forget`: the compiler would keep them), which
 // costs less than the registers they fill.  Where a row takes more than a wavefront, the next row is on its way while this
 // one waits at its barrier.
-template <typename T, int TPR, int NV, int BLOCK, bool TINY>
-__global__ __launch_bounds__(BLOCK) void layernorm_bwd_kernel(const T *__restrict__ g_out, int64_t g_stride,
+template <typename T, int TPR, int NV, bool WIDE, bool TINY>
+__global__ __launch_bounds__(1024) void layernorm_bwd_kernel(const T *__restrict__ g_out, int64_t g_stride,
                                                               const T *__restrict__ x, int64_t x_stride, int64_t M, int C,
                                                               const void *__restrict__ weight, int w_f32,
                                                               const float *__restrict__ mean,
                                                               const float *__restrict__ rstd, T *__restrict__ g_x,
-                                                              float *__restrict__ partial) {
-    constexpr int VEC = Row<T>::VEC, RPB = BLOCK / TPR, LANES = TPR < WAVE ? WAVE : TPR;
-    constexpr bool HOIST = NV * VEC <= 8, TOGETHER = TPR > WAVE, AHEAD = TOGETHER && X_AHEAD;
-    __shared__ float red[TPR > WAVE ? 2 * 2 * (BLOCK / WAVE) : 1];
-    __shared__ float cols[BLOCK > LANES ? 2 * TPR * NV * VEC : 1];
+                                                              float *__restrict__ partial, int waves) {
+    constexpr int VEC = Row<T>::VEC;
+    constexpr bool HOIST = NV * VEC <= 8, AHEAD = WIDE && NV * VEC <= 8;
+    __shared__ float red[WIDE ? 2 * 2 * MAX_WAVES : 1];
+    extern __shared__ float cols[];                           // [NV * VEC][gw, gb][width]
     int slot = 0;
-    const int lane = threadIdx.x % TPR;
+    const Lanes<TPR, WIDE> at_row(waves);
+    const int lane = at_row.lane, width = at_row.width, group = at_row.group;
+    const int lanes = WIDE ? width : WAVE, groups = blockDim.x / lanes, rows = blockDim.x / width;
     const float inv_c = 1.0f / (float)C;
     float w[HOIST ? NV : 1][VEC];
     if constexpr (HOIST) {
 #pragma unroll
         for (int i = 0; i < NV; ++i)
-            nerf::load_weights<TINY, T>(weight, w_f32, nerf::Place<T, TINY>((i * TPR + lane) * VEC, C), 1.0f, w[i]);
+            nerf::load_weights<TINY, T>(weight, w_f32, nerf::Place<T, TINY>((i * width + lane) * VEC, C), 1.0f, w[i]);
     }
     float gw[NV][VEC] = {}, gb[NV][VEC] = {};
     Row<T> px[NV], pg[NV];
@@ -203,31 +226,30 @@ __global__ __launch_bounds__(BLOCK) void layernorm_bwd_kernel(const T *__restric
         r = rstd[row];
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const nerf::Place<T, TINY> at((i * TPR + lane) * VEC, C);
+            const nerf::Place<T, TINY> at((i * width + lane) * VEC, C);
             px[i] = nerf::load_piece<TINY>(x + row * x_stride, at);
             pg[i] = nerf::load_piece<TINY>(g_out + row * g_stride, at);
         }
     };
-    const int64_t first = (int64_t)blockIdx.x * RPB, step = (int64_t)gridDim.x * RPB;
-    const int group = nerf::lane_group<TPR>();
+    const int64_t first = (int64_t)blockIdx.x * rows, step = (int64_t)gridDim.x * rows;
     if (AHEAD) fetch(first + group < M ? first + group : M - 1);
     // (a group beyond the last row goes along to the barriers, with the last row once more and nothing to show for it)
     for (int64_t base = first; base < M; base += step) {
         const bool live = base + group < M;
         const int64_t row = live ? base + group : M - 1;
-        if (!TOGETHER && !live) break;
+        if (!WIDE && !live) break;
         if (!AHEAD) fetch(row);
         float s[2] = {0.0f, 0.0f};
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const nerf::Place<T, TINY> at((i * TPR + lane) * VEC, C);
+            const nerf::Place<T, TINY> at((i * width + lane) * VEC, C);
             if constexpr (!HOIST) nerf::load_weights<TINY, T>(weight, w_f32, at, 1.0f, w[0]);
 #pragma unroll
             for (int j = 0; j < VEC; ++j) {
                 const float g = (float)pg[i].v[j], h = ((float)px[i].v[j] - mu) * r;
                 const float q = at.own(j) ? g * w[HOIST ? i : 0][j] : 0.0f;
-                gw[i][j] = !TOGETHER || live ? fmaf(g, h, gw[i][j]) : gw[i][j];
-                gb[i][j] += !TOGETHER || live ? g : 0.0f;
+                gw[i][j] = !WIDE || live ? fmaf(g, h, gw[i][j]) : gw[i][j];
+                gb[i][j] += !WIDE || live ? g : 0.0f;
                 s[0] += q;
                 s[1] = at.own(j) ? fmaf(q, h, s[1]) : s[1];
             }
@@ -241,13 +263,13 @@ __global__ __launch_bounds__(BLOCK) void layernorm_bwd_kernel(const T *__restric
         }
         const float mu_now = mu, r_now = r;
         if (AHEAD && base + step < M) fetch(base + step + group < M ? base + step + group : M - 1);
-        row_sum<TPR, 2, BLOCK>(s, red, slot);
+        row_sum<TPR, WIDE, 2>(s, red, slot, waves);
         const float c0 = s[0] * inv_c, c1 = s[1] * inv_c;
         const void *w_again = weight;
         if (!HOIST) asm volatile("" : "+s"(w_again));
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const nerf::Place<T, TINY> at((i * TPR + lane) * VEC, C);
+            const nerf::Place<T, TINY> at((i * width + lane) * VEC, C);
             if constexpr (!HOIST) nerf::load_weights<TINY, T>(w_again, w_f32, at, 1.0f, w[0]);
             Row<T> o;
 #pragma unroll
@@ -255,50 +277,51 @@ __global__ __launch_bounds__(BLOCK) void layernorm_bwd_kernel(const T *__restric
                 const float q = (float)g_now[i].v[j] * w[HOIST ? i : 0][j], h = ((float)x_now[i].v[j] - mu_now) * r_now;
                 o.v[j] = (T)(r_now * (q - fmaf(h, c1, c0)));
             }
-            if (!TOGETHER || live) nerf::store_piece<TINY>(g_x + row * C, at, o);
+            if (!WIDE || live) nerf::store_piece<TINY>(g_x + row * C, at, o);
         }
     }
     if (!partial) return;
     float *dst = partial + (int64_t)blockIdx.x * 2 * C;
-    if constexpr (BLOCK == TPR) {
+    // lane groups of a wavefront first, then group after group through LDS
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int j = 0; j < VEC; ++j)
+#pragma unroll
+            for (int d = TPR; d < WAVE; d <<= 1) {
+                gw[i][j] += __shfl_xor(gw[i][j], d, WAVE);
+                gb[i][j] += __shfl_xor(gb[i][j], d, WAVE);
+            }
+    if (groups == 1) {
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const nerf::Place<T, TINY> at((i * TPR + lane) * VEC, C);
+            const nerf::Place<T, TINY> at((i * width + lane) * VEC, C);
 #pragma unroll
             for (int j = 0; j < VEC; ++j)
                 if (at.own(j)) { dst[at.at + j] = gw[i][j]; dst[C + at.at + j] = gb[i][j]; }
         }
-    } else {
-        // lane groups of a wavefront first, then group after group through LDS
+        return;
+    }
+    const int mine = threadIdx.x / lanes;
+    for (int k = 0; k < groups; ++k) {
+        if (mine == k && (int)threadIdx.x - mine * lanes < width) {
 #pragma unroll
-        for (int i = 0; i < NV; ++i)
+            for (int i = 0; i < NV; ++i)
 #pragma unroll
-            for (int j = 0; j < VEC; ++j)
-#pragma unroll
-                for (int d = TPR; d < WAVE; d <<= 1) {
-                    gw[i][j] += __shfl_xor(gw[i][j], d, WAVE);
-                    gb[i][j] += __shfl_xor(gb[i][j], d, WAVE);
+                for (int j = 0; j < VEC; ++j) {
+                    float *c = cols + (i * VEC + j) * 2 * width + lane;
+                    c[0] = k ? c[0] + gw[i][j] : gw[i][j];
+                    c[width] = k ? c[width] + gb[i][j] : gb[i][j];
                 }
-        for (int k = 0; k < BLOCK / LANES; ++k) {
-            if ((int)threadIdx.x / LANES == k && (int)threadIdx.x % LANES < TPR) {
-#pragma unroll
-                for (int i = 0; i < NV; ++i)
-#pragma unroll
-                    for (int j = 0; j < VEC; ++j) {
-                        float *c = cols + (i * VEC + j) * 2 * TPR + lane;
-                        c[0] = k ? c[0] + gw[i][j] : gw[i][j];
-                        c[TPR] = k ? c[TPR] + gb[i][j] : gb[i][j];
-                    }
-            }
-            __syncthreads();
         }
-        for (int k = threadIdx.x; k < TPR * NV * VEC; k += BLOCK) {
-            const int l = k % TPR, ij = k / TPR, j = ij % VEC;
-            const nerf::Place<T, TINY> at(((ij / VEC) * TPR + l) * VEC, C);
-            if (at.own(j)) {
-                dst[at.at + j] = cols[ij * 2 * TPR + l];
-                dst[C + at.at + j] = cols[ij * 2 * TPR + TPR + l];
-            }
+        __syncthreads();
+    }
+    for (int k = threadIdx.x; k < width * NV * VEC; k += blockDim.x) {
+        const int l = k % width, ij = k / width, j = ij % VEC;
+        const nerf::Place<T, TINY> at(((ij / VEC) * width + l) * VEC, C);
+        if (at.own(j)) {
+            dst[at.at + j] = cols[ij * 2 * width + l];
+            dst[C + at.at + j] = cols[ij * 2 * width + width + l];
         }
     }
 }
@@ -360,7 +383,7 @@ __global__ __launch_bounds__(1024) void layernorm_bwd_long_kernel(const T *__res
                 s[1] = at.own(j) ? fmaf(q, ((float)px.v[j] - mu) * r, s[1]) : s[1];
             }
         }
-        row_sum<1024, 2, 1024>(s, red, slot);
+        row_sum<WAVE, true, 2>(s, red, slot, MAX_WAVES);
         const float c0 = s[0] * inv_c, c1 = s[1] * inv_c;
         for (int a = threadIdx.x * VEC; a < C; a += 1024 * VEC) {
             const nerf::Place<T, false> at(a, C);
@@ -405,48 +428,27 @@ __global__ __launch_bounds__(256) void layernorm_bwd_long_columns_kernel(const T
 }
 
 // ------------------------------------------------------------------------------------------------ launches
-constexpr int MAX_REGISTER_ROW = 16384;
+constexpr int MAX_REGISTER_ROW = 16384;      // 1024 threads x 16 values
 
-// f(TPR, NV, BLOCK, TINY) where TPR lanes of NV pieces hold a row of C values
-#define LN_CASE(tpr, values, block, ...)                                                                     \
-    if (C <= (int64_t)(tpr) * (values)) {                                                                    \
-        constexpr int TPR = (tpr), NV = (values) / Row<T>::VEC, BLOCK = (block);                             \
-        constexpr bool TINY = false;                                                                         \
+// f(TPR, NV, WIDE, TINY) where TPR lanes of NV pieces hold a row of C values
+#define LN_USE(tpr, nv, wide, tiny, ...)                                                                     \
+    {                                                                                                        \
+        constexpr int TPR = (tpr), NV = (nv);                                                                \
+        constexpr bool WIDE = (wide), TINY = (tiny);                                                         \
         __VA_ARGS__;                                                                                         \
     }
-#define LN_TINY(block, ...)                                                                                  \
-    if (C < Row<T>::VEC) {                                                                                   \
-        constexpr int TPR = 1, NV = 1, BLOCK = (block);                                                      \
-        constexpr bool TINY = true;                                                                          \
-        __VA_ARGS__;                                                                                         \
+// (fp32 alone: for 16-bit rows the condition in front never holds, and the kernel is not made)
+#define LN_USE_F32(tpr, nv, ...)                                                                             \
+    {                                                                                                        \
+        if constexpr (sizeof(T) == 4) LN_USE(tpr, nv, false, false, __VA_ARGS__)                             \
     }
-// The smallest lane group that holds a row with one piece a lane; then one wavefront with up to 64 values a lane, which
-// needs no barrier; then a workgroup.  Few rows take the workgroup earlier: a row's latency counts, not the barriers.
-#define LN_SHORT(block, ...)                                                                                 \
-    LN_TINY(block, __VA_ARGS__) else LN_CASE(4, Row<T>::VEC, block, __VA_ARGS__)                             \
-    else LN_CASE(8, Row<T>::VEC, block, __VA_ARGS__) else LN_CASE(16, Row<T>::VEC, block, __VA_ARGS__)       \
-    else LN_CASE(32, Row<T>::VEC, block, __VA_ARGS__) else LN_CASE(64, Row<T>::VEC, block, __VA_ARGS__)
-#define LN_FORWARD(...)                                                                                      \
-    LN_SHORT(256, __VA_ARGS__) else LN_CASE(64, 16, 256, __VA_ARGS__)                                        \
-    else if (M >= 1024 && C <= 4096) {                                                                       \
-        LN_CASE(64, 24, 256, __VA_ARGS__) else LN_CASE(64, 32, 256, __VA_ARGS__)                             \
-        else LN_CASE(64, 48, 256, __VA_ARGS__) else LN_CASE(64, 64, 256, __VA_ARGS__)                        \
-    }                                                                                                        \
-    else LN_CASE(256, 8, 256, __VA_ARGS__) else LN_CASE(256, 16, 256, __VA_ARGS__)                           \
-    else LN_CASE(512, 16, 512, __VA_ARGS__) else LN_CASE(1024, 16, 1024, __VA_ARGS__)
-
-// Backward: workgroups as large as the registers of a CU allow, so that few partial rows are left.
-#define LN_BACKWARD(...)                                                                                     \
-    LN_SHORT(1024, __VA_ARGS__) else LN_CASE(64, 8, 1024, __VA_ARGS__) else LN_CASE(64, 16, 512, __VA_ARGS__) \
-    else LN_CASE(256, 8, 1024, __VA_ARGS__) else LN_CASE(256, 16, 1024, __VA_ARGS__)                         \
-    else LN_CASE(512, 16, 1024, __VA_ARGS__) else LN_CASE(1024, 16, 1024, __VA_ARGS__)
-
-// partial rows of the weight's gradient: one per workgroup of the backward pass
-int backward_groups(int64_t M, int64_t C) {
-    const int64_t per = C <= 512 ? 16 : C <= 1024 ? 8 : C <= 4096 ? 4 : C <= 8192 ? 2 : 1;      // rows a workgroup takes at once, at least
-    const int64_t g = (M + per - 1) / per, most = C > MAX_REGISTER_ROW ? 32 : C <= 1024 ? 512 : 256;
-    return (int)(g < 1 ? 1 : g > most ? most : g);
-}
+#define LN_CASE(tpr, nv, ...) if (C <= (int64_t)(tpr) * (nv) * Row<T>::VEC) LN_USE(tpr, nv, false, false, __VA_ARGS__)
+// The smallest lane group that holds a row with one piece a lane, then one wavefront with more: no barrier.
+#define LN_SHORT(...)                                                                                        \
+    if (C < Row<T>::VEC) LN_USE(1, 1, false, true, __VA_ARGS__)                                              \
+    else LN_CASE(1, 1, __VA_ARGS__) else LN_CASE(2, 1, __VA_ARGS__) else LN_CASE(4, 1, __VA_ARGS__)          \
+    else LN_CASE(8, 1, __VA_ARGS__) else LN_CASE(16, 1, __VA_ARGS__)                                         \
+    else LN_CASE(32, 1, __VA_ARGS__) else LN_CASE(64, 1, __VA_ARGS__)
 
 template <typename T>
 void launch_forward(const void *x, int64_t x_stride, int64_t M, int64_t C, const void *weight, const void *bias, int w_f32,
@@ -458,12 +460,46 @@ void launch_forward(const void *x, int64_t x_stride, int64_t M, int64_t C, const
                            x_stride, M, (int)C, weight, bias, w_f32, eps, yt, mean, rstd);
         return;
     }
-    LN_FORWARD({
-        int64_t grid = (M + BLOCK / TPR - 1) / (BLOCK / TPR);
-        if (grid > 256 * 8) grid = 256 * 8;
-        hipLaunchKernelGGL((layernorm_kernel<T, TPR, NV, BLOCK, TINY>), dim3((unsigned)grid), dim3(BLOCK), 0, stream, xt, x_stride,
-                           M, (int)C, weight, bias, w_f32, eps, yt, mean, rstd);
-    })
+    // up to 32 values a lane a wavefront keeps a row to itself; few rows are spread wider, a row's latency counts there
+    constexpr int VEC = Row<T>::VEC;
+    const bool few = M < 1024;
+    // Every workgroup takes its rows once, in the order of the addresses: 1 GB of fp32 rows of 256 at 6.2 TB/s, where 2048
+    // workgroups that stride over the rows reach 5.2.  Short 16-bit rows are too little work for that (4.8 TB/s: the
+    // weights come first): 4 of them one after another, 5.8 TB/s.
+    auto run = [&](auto kernel, int64_t rows, int waves, int per) {
+        const int64_t steps = (M + rows - 1) / rows;
+        if (steps < 4 * 2048) per = 1;
+        const int64_t grid = (steps + per - 1) / per;
+        hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(waves ? waves * WAVE : 256), 0, stream, xt, x_stride, M, (int)C,
+                           weight, bias, w_f32, eps, yt, mean, rstd, waves, per);
+    };
+#define LN_RUN run(layernorm_kernel<T, TPR, NV, WIDE, TINY>, WIDE ? 1 : 256 / TPR, WIDE ? (int)((C + NV * VEC * WAVE - 1) / (NV * VEC * WAVE)) : 0, NV == 1 && VEC == 8 && !WIDE ? 4 : 1)
+    LN_SHORT(LN_RUN) else LN_CASE(64, 2, LN_RUN)
+    else if (few && C <= 8 * 1024) LN_USE(64, 8 / VEC, true, false, LN_RUN)
+    else LN_CASE(64, 3, LN_RUN) else LN_CASE(64, 4, LN_RUN)
+    else if (VEC == 4 && C <= 64 * 24) LN_USE_F32(64, 6, LN_RUN)
+    else if (VEC == 4 && C <= 64 * 32) LN_USE_F32(64, 8, LN_RUN)
+    else LN_USE(64, 16 / VEC, true, false, LN_RUN)
+#undef LN_RUN
+}
+
+// Rows a workgroup of the backward pass has at once, its wavefronts per row (0: lanes of one) and threads.
+struct Shape {
+    int rows, waves, threads, lds;
+};
+
+// Workgroups as large as the registers of a CU allow, so that few partial rows are left.
+template <int TPR, int VALUES, bool WIDE>
+Shape backward_shape(int64_t C) {
+    if (!WIDE) return {1024 / TPR, 0, 1024, 2 * TPR * VALUES * 4};
+    const int waves = (int)((C + VALUES * WAVE - 1) / (VALUES * WAVE)), rows = MAX_WAVES / waves;
+    return {rows, waves, rows * waves * WAVE, rows > 1 ? 2 * waves * WAVE * VALUES * 4 : 0};
+}
+
+// Partial rows of the weight's gradient, one per workgroup: as many workgroups as the chip holds at once.
+int64_t backward_groups(int64_t M, int64_t C, int dtype) {
+    const int64_t most = C > MAX_REGISTER_ROW ? 32 : dtype == NERF_F32 && C <= 256 ? 512 : 256;
+    return M < 1 ? 1 : M > most ? most : M;
 }
 
 template <typename T>
@@ -472,29 +508,37 @@ void launch_backward(const void *g_out, int64_t g_stride, const void *x, int64_t
                      void *g_bias, float *partial, hipStream_t stream) {
     const T *xt = static_cast<const T *>(x), *gt = static_cast<const T *>(g_out);
     T *gx = static_cast<T *>(g_x);
-    const int G = backward_groups(M, C);
     const bool columns = g_weight || g_bias;
+    constexpr int VEC = Row<T>::VEC;
+    int64_t G = M > 0 ? backward_groups(M, C, VEC == 4 ? NERF_F32 : NERF_BF16) : 0;
     if (M > 0 && C > MAX_REGISTER_ROW) {
         hipLaunchKernelGGL(layernorm_bwd_long_kernel<T>, dim3((unsigned)(M < 4096 ? M : 4096)), dim3(1024), 0, stream, gt,
                            g_stride, xt, x_stride, M, (int)C, weight, w_f32, mean, rstd, gx);
         if (columns)
             hipLaunchKernelGGL(layernorm_bwd_long_columns_kernel<T>,
-                               dim3((unsigned)((C + 256 * Row<T>::VEC - 1) / (256 * Row<T>::VEC)), G), dim3(256), 0, stream,
-                               gt, g_stride, xt, x_stride, M, (int)C, mean, rstd, partial);
+                               dim3((unsigned)((C + 256 * Row<T>::VEC - 1) / (256 * Row<T>::VEC)), (unsigned)G), dim3(256), 0,
+                               stream, gt, g_stride, xt, x_stride, M, (int)C, mean, rstd, partial);
     } else if (M > 0) {
-        LN_BACKWARD({
-            hipLaunchKernelGGL((layernorm_bwd_kernel<T, TPR, NV, BLOCK, TINY>), dim3(G), dim3(BLOCK), 0, stream, gt, g_stride, xt,
-                               x_stride, M, (int)C, weight, w_f32, mean, rstd, gx, columns ? partial : nullptr);
-        })
+        auto run = [&](auto kernel, const Shape &s) {
+            const int64_t need = (M + s.rows - 1) / s.rows;
+            if (G > need) G = need;
+            hipLaunchKernelGGL(kernel, dim3((unsigned)G), dim3(s.threads), s.lds, stream, gt, g_stride, xt, x_stride, M, (int)C,
+                               weight, w_f32, mean, rstd, gx, columns ? partial : nullptr, s.waves);
+        };
+#define LN_RUN run(layernorm_bwd_kernel<T, TPR, NV, WIDE, TINY>, backward_shape<TPR, NV * VEC, WIDE>(C))
+        LN_SHORT(LN_RUN)
+        else if (VEC == 4 && C <= 64 * 8) LN_USE_F32(64, 2, LN_RUN)
+        else if (C <= 8 * 1024) LN_USE(64, 8 / VEC, true, false, LN_RUN)
+        else LN_USE(64, 16 / VEC, true, false, LN_RUN)
+#undef LN_RUN
     }
     if (columns) {
         const unsigned grid = (unsigned)((2 * C + 15) / 16);
-        const int rows = M > 0 ? G : 0;
         if (w_f32)
-            hipLaunchKernelGGL(layernorm_columns_kernel<float>, dim3(grid), dim3(1024), 0, stream, partial, rows, C,
+            hipLaunchKernelGGL(layernorm_columns_kernel<float>, dim3(grid), dim3(1024), 0, stream, partial, (int)G, C,
                                static_cast<float *>(g_weight), static_cast<float *>(g_bias));
         else
-            hipLaunchKernelGGL(layernorm_columns_kernel<T>, dim3(grid), dim3(1024), 0, stream, partial, rows, C,
+            hipLaunchKernelGGL(layernorm_columns_kernel<T>, dim3(grid), dim3(1024), 0, stream, partial, (int)G, C,
                                static_cast<T *>(g_weight), static_cast<T *>(g_bias));
     }
 }
@@ -520,7 +564,7 @@ NERF_API int nerf_layernorm(const void *x, int64_t x_stride, int dtype, int64_t 
 
 NERF_API int64_t nerf_layernorm_backward_workspace_bytes(int64_t M, int64_t C) {
     if (!sizes_ok(M, C)) return nerf::fail(NERF_ERR_ARG, "nerf_layernorm_backward_workspace_bytes: size out of range"), -1;
-    return (int64_t)backward_groups(M, C) * 2 * C * 4;
+    return backward_groups(M, C, NERF_F32) * 2 * C * 4;
 }
 
 NERF_API int nerf_layernorm_backward(const void *g_out, int64_t g_stride, const void *x, int64_t x_stride, int dtype, int64_t M,

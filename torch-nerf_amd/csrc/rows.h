@@ -90,18 +90,30 @@ __device__ __forceinline__ void load_weights(const void *w, bool w_f32, const Pl
     }
 }
 
-// Which group of TPR threads this thread is in; a scalar where a wavefront is in one group.
-template <int TPR>
-__device__ __forceinline__ int lane_group() {
-    const int g = threadIdx.x / TPR;
-    return TPR >= WAVE ? __builtin_amdgcn_readfirstlane(g) : g;
+// Sum over groups of WIDTH lanes (a power of two <= 64), every lane gets it.  In the vector ALU alone: inside of 16 lanes by
+// DPP (quad permutes, then mirrors: the quads agree by then, so a mirror is as good as an exchange), across them by gfx950's
+// row and half swaps.  Six steps of ds_bpermute take ten times as long, and a row's sums are in every row's way.
+template <int CTRL>
+__device__ __forceinline__ float dpp_add(float x) {
+    return x + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, 0xf, 0xf, true));
 }
 
-// sum over groups of WIDTH lanes (a power of two <= 64), every lane gets it
 template <int WIDTH>
 __device__ __forceinline__ float lane_sum(float x) {
-#pragma unroll
-    for (int d = 1; d < WIDTH; d <<= 1) x += __shfl_xor(x, d, WAVE);
+    if constexpr (WIDTH >= 2) x = dpp_add<0xB1>(x);          // quad_perm [1, 0, 3, 2]
+    if constexpr (WIDTH >= 4) x = dpp_add<0x4E>(x);          // quad_perm [2, 3, 0, 1]
+    if constexpr (WIDTH >= 8) x = dpp_add<0x141>(x);         // row_half_mirror
+    if constexpr (WIDTH >= 16) x = dpp_add<0x140>(x);        // row_mirror
+    if constexpr (WIDTH >= 32) {
+        const uint32_t u = __builtin_bit_cast(uint32_t, x);
+        const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);     // {rows 0 0 2 2, rows 1 1 3 3}
+        x = __builtin_bit_cast(float, (uint32_t)r[0]) + __builtin_bit_cast(float, (uint32_t)r[1]);
+    }
+    if constexpr (WIDTH >= 64) {
+        const uint32_t u = __builtin_bit_cast(uint32_t, x);
+        const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);     // {low half twice, high half twice}
+        x = __builtin_bit_cast(float, (uint32_t)r[0]) + __builtin_bit_cast(float, (uint32_t)r[1]);
+    }
     return x;
 }
 
