@@ -277,7 +277,10 @@ def test_layernorm_refusals():
 # --------------------------------------------------------------------------- embedding
 EMB = [(1, 1, 1), (1, 5, 3), (7, 3, 16), (64, 10, 5), (300, 100, 48), (513, 1, 33), (1000, 4000, 64), (2000, 17, 257),
        (333, 70001, 12), (40, 300, 2049), (5, 9, 4100), (4097, 2, 8), (16384, 600, 20), (16385, 600, 20), (20000, 90000, 9),
-       (70000, 37, 4)]
+       (70000, 37, 4),
+       (1024, 50, 6), (1025, 50, 6), (32768, 3000, 7), (32769, 3000, 7), (3000, 40000, 1030), (50, 30000, 700),
+       (40000, 100000, 264),
+       (65536, 255, 33), (65537, 64, 33), (65537, 65, 12), (90000, 128, 6), (90000, 129, 6), (700, 255, 2100)]
 
 
 def check_embedding_backward(go, ids, rows, scale, pad, what=""):

@@ -41,10 +41,13 @@ __global__ __launch_bounds__(256) void embedding_kernel(const T *__restrict__ ta
 }
 
 // ------------------------------------------------------------------------------------------------ zeros
-// Rows that no id names are 0, and nobody knows which before the sort: the whole table is cleared, by workgroups that run
-// beside the first sorting launch (the clear is the larger part of a large vocabulary's gradient, and the sort keeps few
-// CUs busy).  The summing launch comes after both.  A workgroup clears `per` pieces next to each other: 268 MB in 43 us
-// (6.2 TB/s); 1024 workgroups striding over the table took 60 us.
+// Rows that no id names are 0.  Clearing a large vocabulary's table is most of its gradient's work, so it goes beside the
+// launches that leave the chip idle: workgroups of the first sorting launches clear the first rows whatever the ids are (as
+// many as the sort takes time for), and workgroups of the summing launch, which can look rows up in the sorted ids, clear
+// those of the others that nothing will be stored to.
+//
+// A workgroup clears `per` pieces next to each other: 268 MB in 43 us (6.2 TB/s); 1024 workgroups striding over the table
+// took 60 us.
 template <typename T>
 __device__ __forceinline__ void clear(T *g_table, int64_t count, int64_t per, int64_t block) {
     Row<T> zero;
@@ -68,8 +71,8 @@ __global__ __launch_bounds__(1024) void embedding_zero_kernel(T *__restrict__ g_
 // digit is (wavefront, step, lane).  `rank` finds a pair's place among the equal digits before it: the lanes that share
 // its digit by one ballot per bit, plus the count its wavefront kept so far.
 constexpr int SORT_THREADS = 1024, SORT_WAVES = SORT_THREADS / WAVE, MAX_DIGIT_BITS = 9, MAX_BINS = 1 << MAX_DIGIT_BITS;
-constexpr int TILE_ITEMS = 4, TILE = SORT_THREADS * TILE_ITEMS;            // several workgroups
-constexpr int ONE_TILE = SORT_THREADS * 16;                                // one workgroup, at most
+constexpr int TILE_ITEMS = 4, TILE = SORT_THREADS * TILE_ITEMS;            // of a pass over many tiles
+constexpr int MERGE_TILES = 32, MERGE_MOST = MERGE_TILES * SORT_THREADS;   // sorted tiles of 1024, merged
 
 __device__ __forceinline__ uint32_t sort_key(const void *ids, int wide, int64_t i, int64_t rows, int64_t padding_idx) {
     const int64_t id = load_id(ids, wide, i);
@@ -94,11 +97,11 @@ struct Tile {
 };
 
 // counts[w][d] <- number of pairs of wavefront w with digit d; place <- number of such pairs before this one
-template <int ITEMS>
+template <int ITEMS, int WAVES = SORT_WAVES>
 __device__ __forceinline__ void rank(Tile<ITEMS> &t, int n_tile, int shift, int bits, uint32_t *counts) {
     const int wave = threadIdx.x / WAVE, lane = threadIdx.x & (WAVE - 1), bins = 1 << bits;
     const uint64_t below = (1ull << lane) - 1;
-    for (int d = threadIdx.x; d < SORT_WAVES * bins; d += SORT_THREADS) counts[d] = 0;
+    for (int d = threadIdx.x; d < WAVES * bins; d += WAVES * WAVE) counts[d] = 0;
     __syncthreads();
     volatile uint32_t *mine = counts + wave * bins;
 #pragma unroll
@@ -118,7 +121,7 @@ __device__ __forceinline__ void rank(Tile<ITEMS> &t, int n_tile, int shift, int 
     __syncthreads();
 }
 
-// Exclusive prefix sum of one value per thread.  sums: SORT_WAVES words.
+// Exclusive prefix sum of one value per thread.  sums: a word per wavefront.
 __device__ __forceinline__ uint32_t block_prefix(uint32_t v, uint32_t *sums) {
     const int wave = threadIdx.x / WAVE, lane = threadIdx.x & (WAVE - 1);
     uint32_t incl = v;
@@ -158,58 +161,73 @@ __device__ __forceinline__ void digit_starts(uint32_t *counts, int bits, uint32_
     __syncthreads();
 }
 
-// All passes in one workgroup (the first; the others clear the table): up to 1024 x ITEMS pairs.  Between two passes the
-// pairs go through LDS.
-template <int ITEMS>
-constexpr int one_lds_bytes(int bits) {
-    return 4 * (SORT_THREADS * ITEMS + (SORT_WAVES << bits) + SORT_WAVES) + 2 * SORT_THREADS * ITEMS;
-}
-
-template <typename T, int ITEMS>
-__global__ __launch_bounds__(SORT_THREADS) void embedding_sort_one_kernel(const void *__restrict__ ids, int wide, int n,
-                                                                          int64_t rows, int64_t padding_idx, int passes,
-                                                                          int bits, uint32_t *__restrict__ keys,
-                                                                          uint32_t *__restrict__ order,
-                                                                          T *__restrict__ g_table, int64_t count, int64_t per) {
-    if (blockIdx.x > 0) {
-        clear(g_table, count, per, blockIdx.x - 1);
+// Up to MERGE_MOST pairs: every workgroup sorts 1024 of them in LDS, all passes, and one more launch merges.
+template <typename T>
+__global__ __launch_bounds__(SORT_THREADS) void embedding_sort_tile_kernel(const void *__restrict__ ids, int wide, int n,
+                                                                           int64_t rows, int64_t padding_idx, int passes,
+                                                                           int bits, int tiles, uint32_t *__restrict__ keys,
+                                                                           uint32_t *__restrict__ order,
+                                                                           T *__restrict__ g_table, int64_t count, int64_t per) {
+    if ((int)blockIdx.x >= tiles) {
+        clear(g_table, count, per, blockIdx.x - tiles);
         return;
     }
-    extern __shared__ uint32_t lds[];
-    uint32_t *sk = lds, *counts = sk + SORT_THREADS * ITEMS, *sums = counts + (SORT_WAVES << bits);
-    uint16_t *sp = reinterpret_cast<uint16_t *>(sums + SORT_WAVES);
-    const int wave = threadIdx.x / WAVE, lane = threadIdx.x & (WAVE - 1);
-    Tile<ITEMS> t;
-#pragma unroll
-    for (int k = 0; k < ITEMS; ++k) {
-        const int i = (wave * ITEMS + k) * WAVE + lane;
-        t.key[k] = i < n ? sort_key(ids, wide, i, rows, padding_idx) : 0;
-        t.pos[k] = i;
-    }
+    __shared__ uint32_t counts[SORT_WAVES * MAX_BINS], sums[SORT_WAVES], sk[SORT_THREADS], sp[SORT_THREADS];
+    const int wave = threadIdx.x / WAVE, begin = blockIdx.x * SORT_THREADS, mine = n - begin < SORT_THREADS ? n - begin : SORT_THREADS;
+    const int i = threadIdx.x;
+    Tile<1> t;
+    t.key[0] = i < mine ? sort_key(ids, wide, begin + i, rows, padding_idx) : 0;
+    t.pos[0] = begin + i;
     for (int p = 0; p < passes; ++p) {
-        rank(t, n, p * bits, bits, counts);
+        rank(t, mine, p * bits, bits, counts);
         digit_starts(counts, bits, sums, nullptr, nullptr, 0);
-#pragma unroll
-        for (int k = 0; k < ITEMS; ++k) {
-            const int i = (wave * ITEMS + k) * WAVE + lane;
-            if (i < n) {
-                const uint32_t to = counts[(wave << bits) + ((t.key[k] >> (p * bits)) & ((1 << bits) - 1))] + t.place[k];
-                sk[to] = t.key[k];
-                sp[to] = (uint16_t)t.pos[k];
-            }
+        if (i < mine) {
+            const uint32_t to = counts[(wave << bits) + ((t.key[0] >> (p * bits)) & ((1 << bits) - 1))] + t.place[0];
+            sk[to] = t.key[0];
+            sp[to] = t.pos[0];
         }
         __syncthreads();
-#pragma unroll
-        for (int k = 0; k < ITEMS; ++k) {
-            const int i = (wave * ITEMS + k) * WAVE + lane;
-            if (i < n) { t.key[k] = sk[i]; t.pos[k] = sp[i]; }
-        }
+        if (i < mine) { t.key[0] = sk[i]; t.pos[0] = sp[i]; }
     }
-#pragma unroll
-    for (int k = 0; k < ITEMS; ++k) {
-        const int i = (wave * ITEMS + k) * WAVE + lane;
-        if (i < n) { keys[i] = t.key[k]; order[i] = t.pos[k]; }
+    if (i < mine) { keys[begin + i] = t.key[0]; order[begin + i] = t.pos[0]; }
+}
+
+// A pair's place among all: its place in its own tile, the pairs of the tiles before that are not larger and those of the
+// tiles behind that are smaller.  All keys are in LDS; the searches of a thread do not wait for each other.
+template <typename T>
+__global__ __launch_bounds__(SORT_THREADS) void embedding_merge_kernel(const uint32_t *__restrict__ keys_in,
+                                                                       const uint32_t *__restrict__ order_in, int n, int tiles,
+                                                                       uint32_t *__restrict__ keys,
+                                                                       uint32_t *__restrict__ order, T *__restrict__ g_table,
+                                                                       int64_t count, int64_t per) {
+    if ((int)blockIdx.x >= tiles) {
+        clear(g_table, count, per, blockIdx.x - tiles);
+        return;
     }
+    extern __shared__ uint32_t all[];
+#pragma unroll 8
+    for (int t = 0; t < tiles; ++t) {
+        const int i = t * SORT_THREADS + threadIdx.x;
+        const uint32_t k = keys_in[i < n ? i : n - 1];
+        all[i] = i < n ? k : ~0u;                            // (nothing: behind all)
+    }
+    const int own = blockIdx.x, i = own * SORT_THREADS + threadIdx.x;
+    const uint32_t pos = i < n ? order_in[i] : 0;
+    __syncthreads();
+    if (i >= n) return;
+    const uint32_t key = all[i];
+    uint32_t place = threadIdx.x;
+#pragma unroll 8
+    for (int t = 0; t < tiles; ++t) {
+        const uint32_t *tile = all + t * SORT_THREADS, limit = key + (t < own ? 1 : 0);      // count the keys below `limit`
+        uint32_t below = 0;
+#pragma unroll
+        for (int step = SORT_THREADS / 2; step > 0; step >>= 1) below += tile[below + step - 1] < limit ? step : 0;
+        below += tile[below] < limit ? 1 : 0;
+        place += t == own ? 0 : below;
+    }
+    keys[place] = key;
+    order[place] = pos;
 }
 
 // One pass over many tiles: counts [digit][tile]; their prefix sums along the tiles and the totals of the digits, one
@@ -303,13 +321,49 @@ __global__ __launch_bounds__(SORT_THREADS) void embedding_sort_move_kernel(const
 // embedding_join_kernel has a row to add up (goes_on).
 constexpr int SUM_THREADS = 256;
 
+// first place in keys[lo, hi) that is not below `limit`; a wavefront looks at 64 places a step
+__device__ __forceinline__ int64_t wave_lower_bound(const uint32_t *keys, int64_t lo, int64_t hi, uint32_t limit) {
+    const int lane = threadIdx.x & (WAVE - 1);
+    while (lo < hi) {
+        const int64_t step = (hi - lo + WAVE - 1) / WAVE, probe = lo + (lane + 1) * step - 1;
+        lo += __popcll(__ballot(probe < hi && keys[probe] < limit)) * step;
+        hi = hi < lo + step - 1 ? hi : lo + step - 1;
+    }
+    return lo;
+}
+
+// Clears those of the rows [first, behind) whose id is not in the sorted keys, in the columns of this workgroup.
+constexpr int MAX_CLEAR_ROWS = SUM_THREADS;
+
+template <typename T>
+__device__ __forceinline__ void clear_absent(T *g_table, int dim, const nerf::Place<T, false> &at, int group, int groups,
+                                             const uint32_t *keys, int64_t n, int64_t first, int64_t behind) {
+    __shared__ bool present[MAX_CLEAR_ROWS];
+    int64_t lo = wave_lower_bound(keys, 0, n, (uint32_t)first), hi = wave_lower_bound(keys, lo, n, (uint32_t)behind);
+    const int64_t row = first + threadIdx.x, end = hi;
+    if (row < behind) {
+        while (lo < hi) {
+            const int64_t m = (lo + hi) >> 1;
+            if (keys[m] < (uint32_t)row) lo = m + 1; else hi = m;
+        }
+        present[threadIdx.x] = lo < end && keys[lo] == (uint32_t)row;
+    }
+    __syncthreads();
+    Row<T> zero;
+#pragma unroll
+    for (int j = 0; j < Row<T>::VEC; ++j) zero.v[j] = (T)0.0f;
+    for (int64_t r = first + group; r < behind; r += groups)
+        if (!present[r - first]) nerf::store_piece<false>(g_table + r * dim, at, zero);
+}
+
 template <typename T, bool TINY>
 __global__ __launch_bounds__(SUM_THREADS) void embedding_sum_kernel(const T *__restrict__ g_out, int64_t n, int dim,
                                                                     const uint32_t *__restrict__ keys,
                                                                     const uint32_t *__restrict__ order, uint32_t rows,
                                                                     float scale, int chunk, int shift,
                                                                     T *__restrict__ g_table, float *__restrict__ partial,
-                                                                    uint32_t *__restrict__ goes_on) {
+                                                                    uint32_t *__restrict__ goes_on, int64_t spans,
+                                                                    int64_t cleared, int clear_rows) {
     constexpr int VEC = Row<T>::VEC, AHEAD = 8;
     // what a chunk has for its neighbours: HEAD -- its first id began before it; THROUGH -- and goes on behind it;
     // TAIL -- its last id begins in it and goes on behind it
@@ -322,6 +376,12 @@ __global__ __launch_bounds__(SUM_THREADS) void embedding_sum_kernel(const T *__r
     const int64_t lo = span + (int64_t)group * chunk, hi = lo + chunk < n ? lo + chunk : n;
     const int column = blockIdx.y * width;
     const nerf::Place<T, TINY> at(column + lane * VEC, dim);
+    if (!TINY && blockIdx.x >= spans) {                       // beside the sums: rows `cleared` and up, clear_rows each
+        const int64_t first = cleared + (blockIdx.x - spans) * clear_rows;
+        clear_absent(g_table, dim, nerf::Place<T, false>(at.at + at.skip, dim), group, groups, keys, n, first,
+                     first + clear_rows < rows ? first + clear_rows : rows);
+        return;
+    }
     if (lo < n && at.live()) {
         uint32_t k[AHEAD], o[AHEAD];
         auto fetch = [&](int64_t i) {
@@ -453,10 +513,178 @@ __global__ __launch_bounds__(256) void embedding_join_kernel(const uint32_t *__r
     }
 }
 
+// ------------------------------------------------------------------------------------------------ few rows
+// A table of a few rows (codes of views, of token types) that a batch hits again and again: no sort over the batch.  A
+// workgroup orders its tile of the batch by id in LDS, sums the runs, and leaves one fp32 partial row per id of the tile,
+// [tile][row][dim], and how often each id occurs, [row][tile]; embedding_few_join_kernel adds the partial rows of an id tile
+// by tile and stores every row of the table, zeros where there is nothing.  Two launches instead of five to seven.
+constexpr int FEW_THREADS = 256, FEW_WAVES = FEW_THREADS / WAVE, FEW_ROWS = FEW_THREADS - 1;
+
+template <typename T, bool TINY, int ITEMS>
+__global__ __launch_bounds__(FEW_THREADS) void embedding_few_kernel(const T *__restrict__ g_out, int64_t n, int dim,
+                                                                    const void *__restrict__ ids, int wide, int rows,
+                                                                    int64_t padding_idx, int bits, int shift,
+                                                                    float *__restrict__ partial,
+                                                                    uint32_t *__restrict__ present) {
+    constexpr int VEC = Row<T>::VEC, AHEAD = 8, PAIRS = FEW_THREADS * ITEMS;
+    constexpr uint32_t HEAD = 1, THROUGH = 2, TAIL = 4;       // as in embedding_sum_kernel
+    __shared__ float part[2][FEW_THREADS * VEC];
+    __shared__ uint32_t counts[FEW_WAVES << 8], sums[FEW_WAVES], kind[FEW_THREADS];
+    __shared__ uint16_t key_of[PAIRS], place_of[PAIRS], first_key[FEW_THREADS];
+    __shared__ int total;
+    const int wave = threadIdx.x / WAVE, lane64 = threadIdx.x & (WAVE - 1), tile = blockIdx.x;
+    const int64_t base = (int64_t)tile * PAIRS;
+    const int mine = n - base < PAIRS ? (int)(n - base) : PAIRS;
+    Tile<ITEMS> t;
+#pragma unroll
+    for (int k = 0; k < ITEMS; ++k) {
+        t.pos[k] = (wave * ITEMS + k) * WAVE + lane64;
+        t.key[k] = (int)t.pos[k] < mine ? sort_key(ids, wide, base + t.pos[k], rows, padding_idx) : 0;
+    }
+    rank<ITEMS, FEW_WAVES>(t, mine, 0, bits, counts);
+    const int bins = 1 << bits, d = threadIdx.x;
+    uint32_t c[FEW_WAVES], here = 0;
+#pragma unroll
+    for (int w = 0; w < FEW_WAVES; ++w) {
+        c[w] = d < bins ? counts[w * bins + d] : 0;
+        here += c[w];
+    }
+    uint32_t start = block_prefix(here, sums);
+    if (d == rows) total = start;                             // ids that give no gradient stand behind the others
+    if (d < rows && blockIdx.y == 0) present[(int64_t)d * gridDim.x + tile] = here;
+#pragma unroll
+    for (int w = 0; w < FEW_WAVES; ++w) {
+        if (d < bins) counts[w * bins + d] = start;
+        start += c[w];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < ITEMS; ++k) {
+        if ((int)t.pos[k] < mine) {
+            const uint32_t to = counts[wave * bins + t.key[k]] + t.place[k];
+            key_of[to] = (uint16_t)t.key[k];
+            place_of[to] = (uint16_t)t.pos[k];
+        }
+    }
+    __syncthreads();
+    const int group = threadIdx.x >> shift, groups = FEW_THREADS >> shift, lane = threadIdx.x & ((1 << shift) - 1);
+    const int width = VEC << shift, column = blockIdx.y * width, all = total, chunk = (all + groups - 1) / groups;
+    const nerf::Place<T, TINY> at(column + lane * VEC, dim);
+    const int lo = group * chunk < all ? group * chunk : all, hi = lo + chunk < all ? lo + chunk : all;
+    float *out = partial + (int64_t)tile * rows * dim;
+    uint32_t mark = 0;
+    if (lo < hi && at.live()) {
+        uint32_t key = key_of[lo];
+        bool begins = lo == 0 || key_of[lo - 1] != key;
+        float sum[VEC] = {};
+        auto flush = [&](bool ends) {
+            if (begins && ends) {
+                float *dst = out + (int64_t)key * dim + at.at;
+#pragma unroll
+                for (int j = 0; j < VEC; ++j)
+                    if (at.own(j)) dst[j] = sum[j];
+            } else {
+                mark |= begins ? TAIL : ends ? HEAD : HEAD | THROUGH;
+                float *dst = part[begins ? 1 : 0] + threadIdx.x * VEC - at.skip;
+#pragma unroll
+                for (int j = 0; j < VEC; ++j)
+                    if (at.own(j)) dst[j] = sum[j];
+            }
+        };
+        if (lane == 0) first_key[group] = (uint16_t)key;
+        for (int i = lo; i < hi; i += AHEAD) {
+            Row<T> r[AHEAD];
+            uint32_t k[AHEAD];
+#pragma unroll
+            for (int u = 0; u < AHEAD; ++u) {
+                const int j = i + u < hi ? i + u : hi - 1;
+                k[u] = key_of[j];
+                r[u] = nerf::load_piece<TINY>(g_out + (base + place_of[j]) * dim, at);
+            }
+#pragma unroll
+            for (int u = 0; u < AHEAD; ++u) {
+                if (i + u >= hi) break;
+                if (k[u] != key) {
+                    flush(true);
+                    key = k[u];
+                    begins = true;
+#pragma unroll
+                    for (int j = 0; j < VEC; ++j) sum[j] = 0.0f;
+                }
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) sum[j] += (float)r[u].v[j];
+            }
+        }
+        flush(hi == all || key_of[hi] != key);
+    }
+    if (lane == 0) kind[group] = mark;
+    __syncthreads();
+    for (int col = threadIdx.x; col < width && column + col < dim; col += FEW_THREADS) {
+        float sum = 0.0f;
+        uint32_t open = 0;                                    // the id that `sum` is of
+        for (int g = 0; g < groups; ++g) {
+            const uint32_t m = kind[g];
+            if (m & HEAD) {
+                sum += part[0][g * width + col];
+                open = first_key[g];
+                if (!(m & THROUGH)) out[(int64_t)open * dim + column + col] = sum;
+            }
+            if (m & TAIL) sum = part[1][g * width + col];
+        }
+    }
+}
+
+// A workgroup adds up 32 columns of a row: the tiles that have it, in order, as a list in LDS, then 8 lanes a partial row,
+// every 32nd of them each, then the 32 sums in order.  (Looking each tile up when its turn comes took 20 us instead of 5 for
+// 768 tiles.)
+template <typename T, bool TINY>
+__global__ __launch_bounds__(256) void embedding_few_join_kernel(const float *__restrict__ partial,
+                                                                 const uint32_t *__restrict__ present, int64_t tiles, int rows,
+                                                                 int dim, float scale, T *__restrict__ g_table) {
+    constexpr int GROUPS = 32, WIDTH = 32;
+    __shared__ float part[GROUPS * WIDTH];
+    __shared__ uint32_t list[256], sums[4];
+    const int group = threadIdx.x >> 3, lane = threadIdx.x & 7, row = blockIdx.x, column = blockIdx.y * WIDTH;
+    const nerf::Place<float, TINY> at(column + lane * 4, dim);
+    float sum[4] = {};
+    for (int64_t first = 0; first < tiles; first += 256) {
+        const int64_t mine = first + threadIdx.x;
+        const bool here = mine < tiles && present[row * tiles + mine] != 0;
+        const uint32_t place = block_prefix(here ? 1 : 0, sums);
+        if (here) list[place] = (uint32_t)threadIdx.x;
+        __syncthreads();
+        const int count = sums[0] + sums[1] + sums[2] + sums[3];
+        if (at.live()) {
+#pragma unroll 4
+            for (int k = group; k < count; k += GROUPS) {
+                const Row<float> r = nerf::load_piece<TINY>(partial + ((first + list[k]) * rows + row) * dim, at);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) sum[j] += r.v[j];
+            }
+        }
+        __syncthreads();
+    }
+    if (at.live()) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (at.own(j)) part[group * WIDTH + at.at + j - column] = sum[j];
+    }
+    __syncthreads();
+    if (threadIdx.x < WIDTH && column + (int)threadIdx.x < dim) {
+        float s = 0.0f;
+#pragma unroll
+        for (int g = 0; g < GROUPS; ++g) s += part[g * WIDTH + threadIdx.x];
+        g_table[(int64_t)row * dim + column + threadIdx.x] = (T)(s * scale);
+    }
+}
+
 // ------------------------------------------------------------------------------------------------ plan
 struct Plan {
+    bool few;                          // embedding_few_kernel: tiles of few_items * FEW_THREADS, no sort
+    int few_items;
     int bits, passes;                  // of the sort
-    int64_t tiles;                     // 0: one workgroup
+    bool merge;                        // sorted tiles of 1024, merged; otherwise passes over many tiles
+    int64_t tiles;
     int shift;                         // 2^shift lanes per row
     int64_t column_tiles;
     int chunk;                         // sorted pairs per lane group
@@ -475,15 +703,31 @@ int lane_shift(int64_t pieces) {
 constexpr int MIN_SUM_SHIFT = 3;
 
 Plan plan_backward(int64_t n, int64_t rows, int64_t dim, int dtype) {
-    Plan p;
+    Plan p = {};
     int bits = 1;
     while (rows >> bits) ++bits;
     p.passes = (bits + MAX_DIGIT_BITS - 1) / MAX_DIGIT_BITS;
     p.bits = (bits + p.passes - 1) / p.passes;
-    p.tiles = n <= ONE_TILE ? 0 : (n + TILE - 1) / TILE;
     const int64_t pieces = (dim * nerf::dtype_bytes(dtype) + 15) / 16;
     p.shift = lane_shift(pieces) > MIN_SUM_SHIFT ? lane_shift(pieces) : MIN_SUM_SHIFT;
     p.column_tiles = (pieces + (1 << p.shift) - 1) >> p.shift;
+    p.merge = n <= MERGE_MOST;
+    // few: what the tiles leave and the join reads, if every id is in every tile, stays a quarter of the batch -- or 8 MB,
+    // where a launch costs more
+    p.few_items = n <= 256 * FEW_THREADS ? 1 : 4;
+    const int64_t pairs = FEW_THREADS * p.few_items, few_tiles = (n + pairs - 1) / pairs;
+    const double left = 2.0 * few_tiles * (rows < pairs ? rows : pairs) * dim * 4, batch = (double)n * dim * nerf::dtype_bytes(dtype);
+    p.few = rows <= FEW_ROWS && left <= (batch / 4 > 8e6 ? batch / 4 : 8e6);
+    int64_t at = 0;
+    auto take = [&](int64_t bytes) { const int64_t r = at; at += (bytes + 255) / 256 * 256; return r; };
+    if (p.few) {
+        p.tiles = few_tiles;
+        p.counts = take(4 * p.tiles * rows);
+        p.partial = take(4 * p.tiles * rows * dim);
+        p.bytes = at;
+        return p;
+    }
+    p.tiles = p.merge ? (n + SORT_THREADS - 1) / SORT_THREADS : (n + TILE - 1) / TILE;
     // about 8 wavefronts per SIMD of the chip, in lane groups; never fewer than 8 pairs a group
     const int64_t groups = ((int64_t)256 * 32 * WAVE >> p.shift) / p.column_tiles;
     int64_t chunk = groups > 0 ? (n + groups - 1) / groups : n;
@@ -491,15 +735,13 @@ Plan plan_backward(int64_t n, int64_t rows, int64_t dim, int dtype) {
     p.chunk = (int)chunk;
     const int64_t span = chunk * (SUM_THREADS >> p.shift);
     p.spans = (n + span - 1) / span;
-    int64_t at = 0;
-    auto take = [&](int64_t bytes) { const int64_t r = at; at += (bytes + 255) / 256 * 256; return r; };
     p.keys = take(4 * n);
     p.order = take(4 * n);
-    const bool twice = p.tiles && p.passes > 1;
+    const bool twice = p.merge ? p.tiles > 1 : p.passes > 1;
     p.keys2 = take(twice ? 4 * n : 0);
     p.order2 = take(twice ? 4 * n : 0);
-    p.counts = take(p.tiles ? 4 * (p.tiles << p.bits) : 0);
-    p.totals = take(p.tiles ? 4 << p.bits : 0);
+    p.counts = take(p.merge ? 0 : 4 * (p.tiles << p.bits));
+    p.totals = take(p.merge ? 0 : 4 << p.bits);
     p.partial = take(p.spans * 2 * dim * 4);
     p.goes_on = take(4 * p.spans);
     p.bytes = at;
@@ -524,60 +766,91 @@ void launch_forward(const void *table, int64_t rows, int64_t row_stride, int64_t
                        row_stride, (int)dim, ids, wide, n, scale, shift, static_cast<T *>(out));
 }
 
-template <typename T, int ITEMS>
-int launch_sort_one(const Plan &p, int64_t clear_blocks, int64_t per, const void *ids, int wide, int64_t n, int64_t rows,
-                    int64_t padding_idx, uint32_t *keys, uint32_t *order, T *g_table, int64_t count,
-                    hipStream_t stream) {
-    static nerf::DeviceMask done;
-    auto kernel = embedding_sort_one_kernel<T, ITEMS>;
-    if (int rc = nerf::ensure_dynamic_lds(reinterpret_cast<const void *>(kernel), one_lds_bytes<ITEMS>(MAX_DIGIT_BITS), done,
-                                          "nerf_embedding_backward"))
-        return rc;
-    hipLaunchKernelGGL(kernel, dim3((unsigned)(1 + clear_blocks)), dim3(SORT_THREADS), one_lds_bytes<ITEMS>(p.bits), stream,
-                       ids, wide, (int)n, rows, padding_idx, p.passes, p.bits, keys, order, g_table, count, per);
-    return NERF_OK;
-}
+// Unconditional clearing of `count` values, shared out to workgroups of SORT_THREADS.
+template <typename T>
+struct Clear {
+    T *at;
+    int64_t count, per, blocks;
+    Clear(T *at_, int64_t count_) : at(at_), count(count_) {
+        const int64_t pieces = (count + Row<T>::VEC - 1) / Row<T>::VEC;
+        blocks = (pieces + SORT_THREADS - 1) / SORT_THREADS;
+        if (blocks > 1024) blocks = 1024;
+        per = blocks ? (pieces + blocks - 1) / blocks : 0;
+    }
+};
+
+// What the chip clears while a sorting launch of some 10 us lasts (65 us a gradient of 16384 x 1024 bf16 into 131072 rows;
+// 70 with 40 MB, 80 with none), and the shortest row that the summing launch clears (a
+// shorter one is less than 32 pieces: looking it up costs more than the store).
+constexpr int64_t CLEAR_BESIDE_SORT = (int64_t)60 << 20, CLEAR_ABSENT_BYTES = 512;
 
 template <typename T>
 int launch_backward(const void *g_out, int dtype, int64_t n, int64_t dim, const void *ids, int wide, int64_t rows, float scale,
                     int64_t padding_idx, void *g_table, char *ws, hipStream_t stream) {
     T *gt = static_cast<T *>(g_table);
-    const int64_t count = rows * dim, pieces = (count + Row<T>::VEC - 1) / Row<T>::VEC;
-    int64_t clear_blocks = (pieces + SORT_THREADS - 1) / SORT_THREADS;
-    if (clear_blocks > 1024) clear_blocks = 1024;
-    const int64_t per = (pieces + clear_blocks - 1) / clear_blocks;
     if (n == 0) {
-        hipLaunchKernelGGL(embedding_zero_kernel<T>, dim3((unsigned)clear_blocks), dim3(SORT_THREADS), 0, stream, gt, count, per);
+        const Clear<T> all(gt, rows * dim);
+        hipLaunchKernelGGL(embedding_zero_kernel<T>, dim3((unsigned)all.blocks), dim3(SORT_THREADS), 0, stream, gt, all.count,
+                           all.per);
         return NERF_OK;
     }
     const Plan p = plan_backward(n, rows, dim, dtype);
     auto words = [&](int64_t offset) { return reinterpret_cast<uint32_t *>(ws + offset); };
     uint32_t *keys = words(p.keys), *order = words(p.order);
     float *partial = reinterpret_cast<float *>(ws + p.partial);
-    if (!p.tiles) {
-        auto sort = n <= SORT_THREADS       ? launch_sort_one<T, 1>
-                    : n <= SORT_THREADS * 4 ? launch_sort_one<T, 4>
-                                            : launch_sort_one<T, 16>;
-        if (int rc = sort(p, clear_blocks, per, ids, wide, n, rows, padding_idx, keys, order, gt, count, stream)) return rc;
+    if (p.few) {
+        const bool tiny = dim < Row<T>::VEC;
+        auto few = p.few_items == 1 ? (tiny ? embedding_few_kernel<T, true, 1> : embedding_few_kernel<T, false, 1>)
+                                    : (tiny ? embedding_few_kernel<T, true, 4> : embedding_few_kernel<T, false, 4>);
+        hipLaunchKernelGGL(few, dim3((unsigned)p.tiles, (unsigned)p.column_tiles), dim3(FEW_THREADS), 0, stream,
+                           static_cast<const T *>(g_out), n, (int)dim, ids, wide, (int)rows, padding_idx, p.bits, p.shift,
+                           partial, words(p.counts));
+        auto join = dim < Row<float>::VEC ? embedding_few_join_kernel<T, true> : embedding_few_join_kernel<T, false>;
+        hipLaunchKernelGGL(join, dim3((unsigned)rows, (unsigned)((dim + 31) / 32)), dim3(256), 0, stream, partial,
+                           words(p.counts), p.tiles, (int)rows, (int)dim, scale, gt);
+        return NERF_OK;
+    }
+    // rows cleared beside the first and the second launch of the sort; the summing launch has the others
+    const int64_t row_bytes = dim * (int64_t)sizeof(T), beside = CLEAR_BESIDE_SORT / row_bytes;
+    const bool second = p.merge && p.tiles > 1;
+    const int64_t first_rows = row_bytes < CLEAR_ABSENT_BYTES ? rows : beside < rows ? beside : rows;
+    const int64_t cleared = second && first_rows + beside < rows ? first_rows + beside : second ? rows : first_rows;
+    const Clear<T> one(gt, first_rows * dim), two(gt + first_rows * dim, (cleared - first_rows) * dim);
+    uint32_t *k[2] = {keys, words(p.keys2)}, *o[2] = {order, words(p.order2)};
+    if (p.merge) {
+        hipLaunchKernelGGL(embedding_sort_tile_kernel<T>, dim3((unsigned)(p.tiles + one.blocks)), dim3(SORT_THREADS), 0, stream,
+                           ids, wide, (int)n, rows, padding_idx, p.passes, p.bits, (int)p.tiles, k[second], o[second], one.at,
+                           one.count, one.per);
+        if (second) {
+            static nerf::DeviceMask done;
+            auto kernel = embedding_merge_kernel<T>;
+            if (int rc = nerf::ensure_dynamic_lds(reinterpret_cast<const void *>(kernel), 4 * MERGE_MOST, done,
+                                                  "nerf_embedding_backward"))
+                return rc;
+            hipLaunchKernelGGL(kernel, dim3((unsigned)(p.tiles + two.blocks)), dim3(SORT_THREADS), 4 * SORT_THREADS * p.tiles,
+                               stream, k[1], o[1], (int)n, (int)p.tiles, keys, order, two.at, two.count, two.per);
+        }
     } else {
         // the last pass has to end in `keys`
-        uint32_t *k[2] = {keys, words(p.keys2)}, *o[2] = {order, words(p.order2)};
         for (int q = 0; q < p.passes; ++q) {
             const int to = (p.passes - 1 - q) & 1;
             const uint32_t *ki = q ? k[to ^ 1] : nullptr, *oi = q ? o[to ^ 1] : nullptr;
-            hipLaunchKernelGGL(embedding_sort_count_kernel<T>, dim3((unsigned)(p.tiles + (q ? 0 : clear_blocks))),
+            hipLaunchKernelGGL(embedding_sort_count_kernel<T>, dim3((unsigned)(p.tiles + (q ? 0 : one.blocks))),
                                dim3(SORT_THREADS), 0, stream, ids, wide, n, rows, padding_idx, ki, q * p.bits, p.bits, p.tiles,
-                               words(p.counts), gt, count, per);
+                               words(p.counts), one.at, one.count, one.per);
             hipLaunchKernelGGL(embedding_sort_scan_kernel, dim3(1u << p.bits), dim3(SORT_THREADS), 0, stream, words(p.counts),
                                p.tiles, words(p.totals));
             hipLaunchKernelGGL(embedding_sort_move_kernel, dim3((unsigned)p.tiles), dim3(SORT_THREADS), 0, stream, ids, wide,
                                n, rows, padding_idx, ki, oi, q * p.bits, p.bits, words(p.totals), words(p.counts), k[to], o[to]);
         }
     }
+    int64_t clear_rows = (128 << 10) / row_bytes;
+    clear_rows = clear_rows < 1 ? 1 : clear_rows > MAX_CLEAR_ROWS ? MAX_CLEAR_ROWS : clear_rows;
+    const int64_t clear_blocks = (rows - cleared + clear_rows - 1) / clear_rows;
     auto sum = dim < Row<T>::VEC ? embedding_sum_kernel<T, true> : embedding_sum_kernel<T, false>;
-    hipLaunchKernelGGL(sum, dim3((unsigned)p.spans, (unsigned)p.column_tiles), dim3(SUM_THREADS), 0, stream,
-                       static_cast<const T *>(g_out), n, (int)dim, keys, order, (uint32_t)rows, scale, p.chunk, p.shift, gt, partial,
-                       words(p.goes_on));
+    hipLaunchKernelGGL(sum, dim3((unsigned)(p.spans + clear_blocks), (unsigned)p.column_tiles), dim3(SUM_THREADS), 0, stream,
+                       static_cast<const T *>(g_out), n, (int)dim, keys, order, (uint32_t)rows, scale, p.chunk, p.shift, gt,
+                       partial, words(p.goes_on), p.spans, cleared, (int)clear_rows);
     if (p.spans > 1) {
         int64_t gy = (dim + 255) / 256;
         auto join = dim < Row<float>::VEC ? embedding_join_kernel<T, true> : embedding_join_kernel<T, false>;
