@@ -311,8 +311,9 @@ int nerf_embedding_backward(const void *g_out, int dtype, int64_t n, int64_t dim
 int nerf_layernorm(const void *x, int64_t x_stride, int dtype, int64_t M, int64_t C, const void *weight, const void *bias,
                    int w_dtype, double eps, void *y, float *mean, float *rstd, nerf_stream_t stream);
 /* g_x (M,C) and, when non-NULL, g_weight / g_bias (C,) of w_dtype, all OVERWRITTEN; mean, rstd as the forward left them.
- * workspace: nerf_layernorm_backward_workspace_bytes(M, C) (may be NULL when neither g_weight nor g_bias is asked for). */
-int64_t nerf_layernorm_backward_workspace_bytes(int64_t M, int64_t C);
+ * workspace: nerf_layernorm_backward_workspace_bytes (0 for a few rows; may be NULL then, and when neither g_weight nor
+ * g_bias is asked for). */
+int64_t nerf_layernorm_backward_workspace_bytes(int64_t M, int64_t C, int dtype);
 int nerf_layernorm_backward(const void *g_out, int64_t g_stride, const void *x, int64_t x_stride, int dtype, int64_t M,
                             int64_t C, const void *weight, int w_dtype, const float *mean, const float *rstd, void *g_x,
                             void *g_weight, void *g_bias, void *workspace, nerf_stream_t stream);

@@ -31,11 +31,13 @@ def test_layernorm_entries_refuse():
     assert back(P, 8, P, 8, 5, 4, 8, P, F32, P, P, P, P, P, P, None) == ARG
     assert back(P, 8, P, 8, F32, 4, 8, P, BF16, P, P, P, P, P, P, None) == ARG
     assert back(P, 7, P, 8, F32, 4, 8, P, F32, P, P, P, P, P, P, None) == ARG
-    assert back(P, 8, P, 8, F32, 4, 8, P, F32, P, P, P, P, P, None, None) == ARG and b"workspace" in lib.nerf_amd_last_error()
+    assert back(P, 8, P, 8, F32, 9000, 8, P, F32, P, P, P, P, P, None, None) == ARG and b"workspace" in lib.nerf_amd_last_error()
     assert back(P, 8, P, 8, F32, 4, 8, P, F32, None, P, P, P, P, P, None) == ARG
-    assert lib.nerf_layernorm_backward_workspace_bytes(4, 0) == -1
-    assert lib.nerf_layernorm_backward_workspace_bytes(-1, 4) == -1
-    assert lib.nerf_layernorm_backward_workspace_bytes(1000, 64) >= 2 * 64 * 4
+    assert lib.nerf_layernorm_backward_workspace_bytes(4, 0, F32) == -1
+    assert lib.nerf_layernorm_backward_workspace_bytes(-1, 4, F32) == -1
+    assert lib.nerf_layernorm_backward_workspace_bytes(4, 4, 9) == -1
+    assert lib.nerf_layernorm_backward_workspace_bytes(4, 64, F16) == 0          # a few rows: one workgroup
+    assert lib.nerf_layernorm_backward_workspace_bytes(100000, 64, F32) >= 2 * 64 * 4
 
 
 def test_embedding_entries_refuse():

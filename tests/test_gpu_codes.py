@@ -137,7 +137,8 @@ def test_layernorm_rows_beyond_a_workgroups_registers(t, C):
 
 
 @pytest.mark.parametrize("t", DTYPES)
-@pytest.mark.parametrize("M,C", [(5000, 7), (20011, 32), (9001, 256), (3001, 300), (2000, 1030), (1500, 4100)])
+@pytest.mark.parametrize("M,C", [(5000, 7), (20011, 32), (9001, 256), (3001, 300), (2000, 1030), (1500, 4100),
+                                 (9, 9000), (300, 9000), (1100, 5), (1025, 2), (4097, 3), (70, 512), (270000, 20), (262145, 130)])
 def test_layernorm_many_rows(t, M, C):
     g = gen(M)
     x, w, b = randn(g, M, C, t=t), randn(g, C, t=t), randn(g, C, t=t)
@@ -224,7 +225,7 @@ def test_layernorm_writes_only_its_rows():
             go = randn(g, M, C, t=t)
             gx = torch.full((M * C + 40,), 7.0, device="cuda", dtype=t)
             cols = torch.full((2, C + 10), 7.0, device="cuda")
-            ws = torch.empty(lib.nerf_layernorm_backward_workspace_bytes(M, C), dtype=torch.uint8, device="cuda")
+            ws = torch.empty(lib.nerf_layernorm_backward_workspace_bytes(M, C, CODE[t]) + 16, dtype=torch.uint8, device="cuda")
             rc = lib.nerf_layernorm_backward(go.data_ptr(), C, x.data_ptr(), C, CODE[t], M, C, None, 0, mu.data_ptr(),
                                              r.data_ptr(), gx.data_ptr() + 21 * size, cols[0].data_ptr() + 20,
                                              cols[1].data_ptr() + 20, ws.data_ptr(), torch.cuda.current_stream().cuda_stream)

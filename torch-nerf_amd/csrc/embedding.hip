@@ -19,24 +19,35 @@ __device__ __forceinline__ int64_t load_id(const void *ids, int wide, int64_t i)
     return wide ? static_cast<const int64_t *>(ids)[i] : (int64_t) static_cast<const int32_t *>(ids)[i];
 }
 
-// 2^shift lanes share a row and step through its pieces
-template <typename T, bool TINY>
-__global__ __launch_bounds__(256) void embedding_kernel(const T *__restrict__ table, int64_t rows, int64_t row_stride,
-                                                        int dim, const void *__restrict__ ids, int wide, int64_t n,
-                                                        float scale, int shift, T *__restrict__ out) {
+// Rows of up to 256 pieces stand in a workgroup lane by lane, whatever their length: thread t has piece t % pieces of row
+// t / pieces (t < 1024 and pieces <= 256: `magic` = ceil(2^20 / pieces) divides exactly).  Longer rows take a workgroup each,
+// STEPS pieces of a lane on their way at once.  Every workgroup takes its rows once, in the order of the output's addresses.
+template <typename T, bool TINY, int STEPS>
+__global__ __launch_bounds__(1024) void embedding_kernel(const T *__restrict__ table, int64_t rows, int64_t row_stride,
+                                                         int dim, const void *__restrict__ ids, int wide, int64_t n,
+                                                         float scale, int pieces, uint32_t magic, int per,
+                                                         T *__restrict__ out) {
     constexpr int VEC = Row<T>::VEC;
-    const int per = 256 >> shift, lane = threadIdx.x & ((1 << shift) - 1);
-    for (int64_t i = (int64_t)blockIdx.x * per + (threadIdx.x >> shift); i < n; i += (int64_t)gridDim.x * per) {
-        const int64_t id = load_id(ids, wide, i);
-        const bool known = id >= 0 && id < rows;
-        const T *src = table + (known ? id : 0) * row_stride;
-        for (int a = (((int)blockIdx.y << shift) + lane) * VEC; a < dim; a += ((int)gridDim.y << shift) * VEC) {
-            const nerf::Place<T, TINY> at(a, dim);
-            Row<T> r = nerf::load_piece<TINY>(src, at);
+    const int mine = STEPS > 1 ? 0 : (int)(threadIdx.x * magic >> 20), lane = (int)threadIdx.x - mine * pieces;
+    const int64_t i = (int64_t)blockIdx.x * per + mine;
+    if (i >= n || mine >= per) return;
+    const int64_t id = load_id(ids, wide, i);
+    const bool known = id >= 0 && id < rows;
+    const T *src = table + (known ? id : 0) * row_stride;
+    T *dst = out + i * dim;
+    const float factor = known ? scale : __builtin_nanf("");
+    const int step = blockDim.x * VEC;
+    for (int first = lane * VEC; first < dim; first += STEPS * step) {
+        Row<T> r[STEPS];
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) r.v[j] = (T)(known ? (float)r.v[j] * scale : __builtin_nanf(""));
-            nerf::store_piece<TINY>(out + i * dim, at, r);
+        for (int k = 0; k < STEPS; ++k) r[k] = nerf::load_piece<TINY>(src, nerf::Place<T, TINY>(first + k * step, dim));
+#pragma unroll
+        for (int k = 0; k < STEPS; ++k) {
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) r[k].v[j] = (T)((float)r[k].v[j] * factor);
+            nerf::store_piece<TINY>(dst, nerf::Place<T, TINY>(first + k * step, dim), r[k]);
         }
+        if (STEPS == 1) break;
     }
 }
 
@@ -722,6 +733,11 @@ Plan plan_backward(int64_t n, int64_t rows, int64_t dim, int dtype) {
     auto take = [&](int64_t bytes) { const int64_t r = at; at += (bytes + 255) / 256 * 256; return r; };
     if (p.few) {
         p.tiles = few_tiles;
+        // a small batch of long rows: fewer lanes a row, so that more workgroups share the columns
+        while (p.shift > MIN_SUM_SHIFT && p.tiles * p.column_tiles < 512) {
+            --p.shift;
+            p.column_tiles = (pieces + (1 << p.shift) - 1) >> p.shift;
+        }
         p.counts = take(4 * p.tiles * rows);
         p.partial = take(4 * p.tiles * rows * dim);
         p.bytes = at;
@@ -756,14 +772,13 @@ template <typename T>
 void launch_forward(const void *table, int64_t rows, int64_t row_stride, int64_t dim, const void *ids, int wide, int64_t n,
                     float scale, void *out, hipStream_t stream) {
     const int64_t pieces = (dim + Row<T>::VEC - 1) / Row<T>::VEC;
-    const int shift = lane_shift(pieces);
-    const int64_t per = 256 >> shift;
-    int64_t gx = (n + per - 1) / per, gy = (pieces + (1 << shift) - 1) >> shift;
-    if (gx > 256 * 16) gx = 256 * 16;
-    if (gy > 64) gy = 64;
-    auto kernel = dim < Row<T>::VEC ? embedding_kernel<T, true> : embedding_kernel<T, false>;
-    hipLaunchKernelGGL(kernel, dim3((unsigned)gx, (unsigned)gy), dim3(256), 0, stream, static_cast<const T *>(table), rows,
-                       row_stride, (int)dim, ids, wide, n, scale, shift, static_cast<T *>(out));
+    const bool packed = pieces <= 256;
+    const int64_t per = packed ? 1024 / pieces : 1;
+    const unsigned threads = packed ? (unsigned)((per * pieces + WAVE - 1) / WAVE * WAVE) : 256;
+    auto kernel = dim < Row<T>::VEC ? embedding_kernel<T, true, 1> : packed ? embedding_kernel<T, false, 1> : embedding_kernel<T, false, 4>;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)((n + per - 1) / per)), dim3(threads), 0, stream, static_cast<const T *>(table),
+                       rows, row_stride, (int)dim, ids, wide, n, scale, (int)pieces,
+                       (uint32_t)(((1 << 20) + pieces - 1) / pieces), (int)per, static_cast<T *>(out));
 }
 
 // Unconditional clearing of `count` values, shared out to workgroups of SORT_THREADS.

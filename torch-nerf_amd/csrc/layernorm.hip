@@ -191,6 +191,14 @@ __global__ __launch_bounds__(1024) void layernorm_long_kernel(const T *__restric
 }
 
 // ------------------------------------------------------------------------------------------------ backward
+template <typename T>
+__device__ __forceinline__ void store_column(void *out, int f32, int c, float v) {
+    if (f32)
+        static_cast<float *>(out)[c] = v;
+    else
+        static_cast<T *>(out)[c] = (T)v;
+}
+
 // Every workgroup walks its rows with the column sums of gw and gb in registers and leaves one partial row
 // [2][C] (fp32) of them; layernorm_columns_kernel adds the partials in a fixed order: no atomics, the same bits every run.
 // A row stays in registers as it was read; h and q are made from it twice (`forget`: the compiler would keep them), which
@@ -202,11 +210,12 @@ __global__ __launch_bounds__(1024) void layernorm_bwd_kernel(const T *__restrict
                                                               const void *__restrict__ weight, int w_f32,
                                                               const float *__restrict__ mean,
                                                               const float *__restrict__ rstd, T *__restrict__ g_x,
-                                                              float *__restrict__ partial, int waves) {
+                                                              float *__restrict__ partial, void *__restrict__ g_weight,
+                                                              void *__restrict__ g_bias, int waves, int64_t per) {
     constexpr int VEC = Row<T>::VEC;
     constexpr bool HOIST = NV * VEC <= 8, AHEAD = WIDE && NV * VEC <= 8;
     __shared__ float red[WIDE ? 2 * 2 * MAX_WAVES : 1];
-    extern __shared__ float cols[];                           // [NV * VEC][gw, gb][width]
+    extern __shared__ float cols[];                           // the groups' column sums
     int slot = 0;
     const Lanes<TPR, WIDE> at_row(waves);
     const int lane = at_row.lane, width = at_row.width, group = at_row.group;
@@ -231,12 +240,14 @@ __global__ __launch_bounds__(1024) void layernorm_bwd_kernel(const T *__restrict
             pg[i] = nerf::load_piece<TINY>(g_out + row * g_stride, at);
         }
     };
-    const int64_t first = (int64_t)blockIdx.x * rows, step = (int64_t)gridDim.x * rows;
-    if (AHEAD) fetch(first + group < M ? first + group : M - 1);
+    // per > 0: so many steps of rows next to each other; 0: every gridDim.x-th step
+    const int64_t first = (int64_t)blockIdx.x * (per ? per : 1) * rows, step = per ? rows : (int64_t)gridDim.x * rows;
+    const int64_t end = per && first + per * rows < M ? first + per * rows : M;
+    if (AHEAD) fetch(first + group < end ? first + group : end - 1);
     // (a group beyond the last row goes along to the barriers, with the last row once more and nothing to show for it)
-    for (int64_t base = first; base < M; base += step) {
-        const bool live = base + group < M;
-        const int64_t row = live ? base + group : M - 1;
+    for (int64_t base = first; base < end; base += step) {
+        const bool live = base + group < end;
+        const int64_t row = live ? base + group : end - 1;
         if (!WIDE && !live) break;
         if (!AHEAD) fetch(row);
         float s[2] = {0.0f, 0.0f};
@@ -262,7 +273,7 @@ __global__ __launch_bounds__(1024) void layernorm_bwd_kernel(const T *__restrict
             if (!HOIST) { forget(x_now[i]); forget(g_now[i]); }
         }
         const float mu_now = mu, r_now = r;
-        if (AHEAD && base + step < M) fetch(base + step + group < M ? base + step + group : M - 1);
+        if (AHEAD && base + step < end) fetch(base + step + group < end ? base + step + group : end - 1);
         row_sum<TPR, WIDE, 2>(s, red, slot, waves);
         const float c0 = s[0] * inv_c, c1 = s[1] * inv_c;
         const void *w_again = weight;
@@ -280,9 +291,19 @@ __global__ __launch_bounds__(1024) void layernorm_bwd_kernel(const T *__restrict
             if (!WIDE || live) nerf::store_piece<TINY>(g_x + row * C, at, o);
         }
     }
-    if (!partial) return;
-    float *dst = partial + (int64_t)blockIdx.x * 2 * C;
-    // lane groups of a wavefront first, then group after group through LDS
+    if (!g_weight && !g_bias) return;
+    // one workgroup alone has the gradients themselves
+    auto put = [&](int c, float w_sum, float b_sum) {
+        if (gridDim.x > 1) {
+            float *dst = partial + (int64_t)blockIdx.x * 2 * C;
+            dst[c] = w_sum;
+            dst[C + c] = b_sum;
+        } else {
+            if (g_weight) store_column<T>(g_weight, w_f32, c, w_sum);
+            if (g_bias) store_column<T>(g_bias, w_f32, c, b_sum);
+        }
+    };
+    // lane groups of a wavefront first, then the groups of the workgroup through LDS, in order
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
@@ -298,31 +319,32 @@ __global__ __launch_bounds__(1024) void layernorm_bwd_kernel(const T *__restrict
             const nerf::Place<T, TINY> at((i * width + lane) * VEC, C);
 #pragma unroll
             for (int j = 0; j < VEC; ++j)
-                if (at.own(j)) { dst[at.at + j] = gw[i][j]; dst[C + at.at + j] = gb[i][j]; }
+                if (at.own(j)) put(at.at + j, gw[i][j], gb[i][j]);
         }
         return;
     }
-    const int mine = threadIdx.x / lanes;
-    for (int k = 0; k < groups; ++k) {
-        if (mine == k && (int)threadIdx.x - mine * lanes < width) {
+    // [group][NV * VEC][gw, gb][width]
+    const int mine = threadIdx.x / lanes, size = NV * VEC * 2 * width;
+    if ((int)threadIdx.x - mine * lanes < width) {
 #pragma unroll
-            for (int i = 0; i < NV; ++i)
+        for (int i = 0; i < NV; ++i)
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) {
-                    float *c = cols + (i * VEC + j) * 2 * width + lane;
-                    c[0] = k ? c[0] + gw[i][j] : gw[i][j];
-                    c[width] = k ? c[width] + gb[i][j] : gb[i][j];
-                }
-        }
-        __syncthreads();
+            for (int j = 0; j < VEC; ++j) {
+                float *c = cols + mine * size + (i * VEC + j) * 2 * width + lane;
+                c[0] = gw[i][j];
+                c[width] = gb[i][j];
+            }
     }
+    __syncthreads();
     for (int k = threadIdx.x; k < width * NV * VEC; k += blockDim.x) {
         const int l = k % width, ij = k / width, j = ij % VEC;
         const nerf::Place<T, TINY> at(((ij / VEC) * width + l) * VEC, C);
-        if (at.own(j)) {
-            dst[at.at + j] = cols[ij * 2 * width + l];
-            dst[C + at.at + j] = cols[ij * 2 * width + width + l];
+        float w_sum = 0.0f, b_sum = 0.0f;
+        for (int g = 0; g < groups; ++g) {
+            w_sum += cols[g * size + ij * 2 * width + l];
+            b_sum += cols[g * size + ij * 2 * width + width + l];
         }
+        if (at.own(j)) put(at.at + j, w_sum, b_sum);
     }
 }
 
@@ -483,23 +505,48 @@ void launch_forward(const void *x, int64_t x_stride, int64_t M, int64_t C, const
 #undef LN_RUN
 }
 
-// Rows a workgroup of the backward pass has at once, its wavefronts per row (0: lanes of one) and threads.
-struct Shape {
-    int rows, waves, threads, lds;
+// How the backward pass walks the rows.
+struct Walk {
+    int rows, waves, threads;          // of a workgroup: rows at once, wavefronts per row (0: lanes of one), threads
+    int64_t groups, per;               // workgroups = partial rows of the weight's gradient; see the kernel
+    bool alone;                        // one workgroup, which stores the gradients itself
 };
 
-// Workgroups as large as the registers of a CU allow, so that few partial rows are left.
-template <int TPR, int VALUES, bool WIDE>
-Shape backward_shape(int64_t C) {
-    if (!WIDE) return {1024 / TPR, 0, 1024, 2 * TPR * VALUES * 4};
-    const int waves = (int)((C + VALUES * WAVE - 1) / (VALUES * WAVE)), rows = MAX_WAVES / waves;
-    return {rows, waves, rows * waves * WAVE, rows > 1 ? 2 * waves * WAVE * VALUES * 4 : 0};
-}
-
-// Partial rows of the weight's gradient, one per workgroup: as many workgroups as the chip holds at once.
-int64_t backward_groups(int64_t M, int64_t C, int dtype) {
-    const int64_t most = C > MAX_REGISTER_ROW ? 32 : dtype == NERF_F32 && C <= 256 ? 512 : 256;
-    return M < 1 ? 1 : M > most ? most : M;
+// Workgroups as large as the registers of a CU allow, so that few partial rows are left: as many as the chip holds at once,
+// striding over the rows.  Short fp32 rows in large numbers are quicker in the order of the addresses, 16 steps a workgroup
+// (786432 x 256: 470 us instead of 500); 16-bit rows are not (239 us instead of 234 at the same bytes).
+Walk plan_walk(int64_t M, int64_t C, int dtype) {
+    // up to so many steps of one workgroup, a few us each, are quicker than a second launch for the columns
+    constexpr int64_t ONE_WORKGROUP = 4, STRIDING = 256, IN_ORDER = 16, IN_ORDER_FROM = 1024, IN_ORDER_MOST = 4096;
+    const int vec = 16 / nerf::dtype_bytes(dtype);
+    Walk w = {};
+    if (C > MAX_REGISTER_ROW) {
+        w.groups = M < 1 ? 1 : M > 32 ? 32 : M;              // of layernorm_bwd_long_columns_kernel
+        return w;
+    }
+    if (C <= (dtype == NERF_F32 ? 512 : WAVE * vec)) {
+        int lanes = 1;
+        while (lanes < WAVE && lanes * vec < C) lanes <<= 1;
+        w.rows = 1024 / lanes;
+        w.threads = 1024;
+    } else {
+        const int values = C <= 8 * 1024 ? 8 : 16;
+        w.waves = (int)((C + values * WAVE - 1) / (values * WAVE));
+        w.rows = MAX_WAVES / w.waves;
+        w.threads = w.rows * w.waves * WAVE;
+    }
+    const int64_t steps = (M + w.rows - 1) / w.rows;
+    w.alone = steps <= ONE_WORKGROUP;
+    if (w.alone) {
+        w.groups = 1;
+    } else if (dtype == NERF_F32 && w.waves == 0 && steps >= IN_ORDER * IN_ORDER_FROM) {
+        w.per = (steps + IN_ORDER_MOST - 1) / IN_ORDER_MOST;
+        if (w.per < IN_ORDER) w.per = IN_ORDER;
+        w.groups = (steps + w.per - 1) / w.per;
+    } else {
+        w.groups = steps < STRIDING ? steps : STRIDING;
+    }
+    return w;
 }
 
 template <typename T>
@@ -510,35 +557,36 @@ void launch_backward(const void *g_out, int64_t g_stride, const void *x, int64_t
     T *gx = static_cast<T *>(g_x);
     const bool columns = g_weight || g_bias;
     constexpr int VEC = Row<T>::VEC;
-    int64_t G = M > 0 ? backward_groups(M, C, VEC == 4 ? NERF_F32 : NERF_BF16) : 0;
+    const Walk walk = plan_walk(M, C, VEC == 4 ? NERF_F32 : NERF_BF16);
     if (M > 0 && C > MAX_REGISTER_ROW) {
         hipLaunchKernelGGL(layernorm_bwd_long_kernel<T>, dim3((unsigned)(M < 4096 ? M : 4096)), dim3(1024), 0, stream, gt,
                            g_stride, xt, x_stride, M, (int)C, weight, w_f32, mean, rstd, gx);
         if (columns)
             hipLaunchKernelGGL(layernorm_bwd_long_columns_kernel<T>,
-                               dim3((unsigned)((C + 256 * Row<T>::VEC - 1) / (256 * Row<T>::VEC)), (unsigned)G), dim3(256), 0,
-                               stream, gt, g_stride, xt, x_stride, M, (int)C, mean, rstd, partial);
+                               dim3((unsigned)((C + 256 * VEC - 1) / (256 * VEC)), (unsigned)walk.groups), dim3(256), 0, stream, gt,
+                               g_stride, xt, x_stride, M, (int)C, mean, rstd, partial);
     } else if (M > 0) {
-        auto run = [&](auto kernel, const Shape &s) {
-            const int64_t need = (M + s.rows - 1) / s.rows;
-            if (G > need) G = need;
-            hipLaunchKernelGGL(kernel, dim3((unsigned)G), dim3(s.threads), s.lds, stream, gt, g_stride, xt, x_stride, M, (int)C,
-                               weight, w_f32, mean, rstd, gx, columns ? partial : nullptr, s.waves);
+        // LDS: the column sums of every group of lanes that has one, where there is more than one group
+        auto run = [&](auto kernel, int lanes, int values) {
+            const int lds = lanes < walk.threads ? (lanes < WAVE ? walk.threads / WAVE : walk.threads / lanes) * lanes * values * 8 : 0;
+            hipLaunchKernelGGL(kernel, dim3((unsigned)walk.groups), dim3(walk.threads), lds, stream, gt, g_stride, xt, x_stride, M,
+                               (int)C, weight, w_f32, mean, rstd, gx, partial, g_weight, g_bias, walk.waves,
+                               walk.per);
         };
-#define LN_RUN run(layernorm_bwd_kernel<T, TPR, NV, WIDE, TINY>, backward_shape<TPR, NV * VEC, WIDE>(C))
+#define LN_RUN run(layernorm_bwd_kernel<T, TPR, NV, WIDE, TINY>, WIDE ? walk.waves * WAVE : TPR, NV * VEC)
         LN_SHORT(LN_RUN)
         else if (VEC == 4 && C <= 64 * 8) LN_USE_F32(64, 2, LN_RUN)
         else if (C <= 8 * 1024) LN_USE(64, 8 / VEC, true, false, LN_RUN)
         else LN_USE(64, 16 / VEC, true, false, LN_RUN)
 #undef LN_RUN
     }
-    if (columns) {
+    if (columns && !(walk.alone && M > 0)) {
         const unsigned grid = (unsigned)((2 * C + 15) / 16);
         if (w_f32)
-            hipLaunchKernelGGL(layernorm_columns_kernel<float>, dim3(grid), dim3(1024), 0, stream, partial, (int)G, C,
+            hipLaunchKernelGGL(layernorm_columns_kernel<float>, dim3(grid), dim3(1024), 0, stream, partial, M > 0 ? (int)walk.groups : 0, C,
                                static_cast<float *>(g_weight), static_cast<float *>(g_bias));
         else
-            hipLaunchKernelGGL(layernorm_columns_kernel<T>, dim3(grid), dim3(1024), 0, stream, partial, (int)G, C,
+            hipLaunchKernelGGL(layernorm_columns_kernel<T>, dim3(grid), dim3(1024), 0, stream, partial, M > 0 ? (int)walk.groups : 0, C,
                                static_cast<T *>(g_weight), static_cast<T *>(g_bias));
     }
 }
@@ -562,9 +610,10 @@ NERF_API int nerf_layernorm(const void *x, int64_t x_stride, int dtype, int64_t 
     return nerf::check_launch("nerf_layernorm");
 }
 
-NERF_API int64_t nerf_layernorm_backward_workspace_bytes(int64_t M, int64_t C) {
-    if (!sizes_ok(M, C)) return nerf::fail(NERF_ERR_ARG, "nerf_layernorm_backward_workspace_bytes: size out of range"), -1;
-    return backward_groups(M, C, NERF_F32) * 2 * C * 4;
+NERF_API int64_t nerf_layernorm_backward_workspace_bytes(int64_t M, int64_t C, int dtype) {
+    if (!nerf::known_dtype(dtype) || !sizes_ok(M, C)) return nerf::fail(NERF_ERR_ARG, "nerf_layernorm_backward_workspace_bytes: size out of range"), -1;
+    const Walk w = plan_walk(M, C, dtype);
+    return w.alone || M == 0 ? 0 : w.groups * 2 * C * 4;
 }
 
 NERF_API int nerf_layernorm_backward(const void *g_out, int64_t g_stride, const void *x, int64_t x_stride, int dtype, int64_t M,
@@ -574,7 +623,8 @@ NERF_API int nerf_layernorm_backward(const void *g_out, int64_t g_stride, const 
     NERF_REQUIRE(w_dtype == dtype || w_dtype == NERF_F32, "nerf_layernorm_backward: weights are of x's dtype or fp32");
     NERF_REQUIRE(sizes_ok(M, C), "nerf_layernorm_backward: size out of range");
     NERF_REQUIRE(M == 0 || (g_out && x && mean && rstd && g_x), "nerf_layernorm_backward: null pointer");
-    NERF_REQUIRE(!(g_weight || g_bias) || M == 0 || workspace, "nerf_layernorm_backward: workspace missing");
+    NERF_REQUIRE(!(g_weight || g_bias) || workspace || nerf_layernorm_backward_workspace_bytes(M, C, dtype) == 0,
+                 "nerf_layernorm_backward: workspace missing");
     NERF_REQUIRE(M <= 1 || (x_stride >= C && g_stride >= C), "nerf_layernorm_backward: rows overlap (stride < C)");
     NERF_FOR_DTYPE(dtype, T, launch_backward<T>(g_out, g_stride, x, x_stride, M, C, weight, w_dtype == NERF_F32, mean, rstd,
                                                 g_x, g_weight, g_bias, static_cast<float *>(workspace),

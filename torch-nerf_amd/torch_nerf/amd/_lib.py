@@ -72,7 +72,7 @@ SIGNATURES = {
     "nerf_embedding_backward_workspace_bytes": (_c_i64, [_c_i64, _c_i64, _c_i64, _c_int]),
     "nerf_embedding_backward": (_c_int, [_p, _c_int, _c_i64, _c_i64, _p, _c_int, _c_i64, _c_f, _c_i64, _p, _p, _p]),
     "nerf_layernorm": (_c_int, [_p, _c_i64, _c_int, _c_i64, _c_i64, _p, _p, _c_int, _c_d, _p, _p, _p, _p]),
-    "nerf_layernorm_backward_workspace_bytes": (_c_i64, [_c_i64, _c_i64]),
+    "nerf_layernorm_backward_workspace_bytes": (_c_i64, [_c_i64, _c_i64, _c_int]),
     "nerf_layernorm_backward": (_c_int, [_p, _c_i64, _p, _c_i64, _c_int, _c_i64, _c_i64, _p, _c_int, _p, _p, _p, _p, _p,
                                          _p, _p]),
     "nerf_dropout": (_c_int, [_p, _p, _c_int, _c_i64, _c_d, ctypes.c_uint64, _p, _c_i64, _p, _p]),

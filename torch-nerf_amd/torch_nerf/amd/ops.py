@@ -744,12 +744,12 @@ def embedding_backward(g_out: torch.Tensor, ids: torch.Tensor, num_rows: int, sc
         raise ValueError(f"num_rows {num_rows} must be positive, padding_idx {padding_idx} None or one of its rows")
     lib = _lib.load()
     g_out, ids = g_out.contiguous(), ids.contiguous()
-    n, dim, dev = ids.numel(), g_out.shape[-1], g_out.device
+    n, dim = ids.numel(), g_out.shape[-1]
     size = lib.nerf_embedding_backward_workspace_bytes(n, num_rows, dim, code)
     if size < 0:
         _lib.check(1, "nerf_embedding_backward_workspace_bytes")
-    g_table = torch.empty((num_rows, dim), dtype=g_out.dtype, device=dev)
-    ws = torch.empty((size,), dtype=torch.uint8, device=dev)
+    g_table = g_out.new_empty((num_rows, dim))
+    ws = g_out.new_empty((size,), dtype=torch.uint8)
     _enqueue(g_out.get_device(), "nerf_embedding_backward", lib.nerf_embedding_backward, g_out.data_ptr(), code, n, dim,
              ids.data_ptr(), wide, num_rows, float(scale), pad, g_table.data_ptr(), ws.data_ptr())
     return g_table
@@ -773,16 +773,17 @@ class EmbeddingFunction(torch.autograd.Function):
 
 def _norm_weights(x: torch.Tensor, weight, bias):
     """(weight, bias, element type of both): x's or fp32, None where absent."""
-    C, dtype = x.shape[-1], None
-    out = []
-    for name, t in (("weight", weight), ("bias", bias)):
-        if t is not None:
-            dtype = getattr(t, "dtype", None) if dtype is None else dtype
-            if dtype != x.dtype and dtype != torch.float32:
-                raise ValueError(f"{name}: expected {x.dtype} or float32, got {dtype}")
-            t = _like(t, name, x, "x", shape=(C,), dtype=dtype)
-        out.append(t)
-    return out[0], out[1], dtype or x.dtype
+    if weight is None and bias is None:
+        return None, None, x.dtype
+    dtype = getattr(bias if weight is None else weight, "dtype", None)
+    if dtype != x.dtype and dtype != torch.float32:
+        raise ValueError(f"weight, bias: expected {x.dtype} or float32, got {dtype}")
+    shape = x.shape[-1:]
+    if weight is not None:
+        weight = _like(weight, "weight", x, "x", shape, dtype)
+    if bias is not None:
+        bias = _like(bias, "bias", x, "x", shape, dtype)
+    return weight, bias, dtype
 
 
 def layernorm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
@@ -824,17 +825,18 @@ def layernorm_backward(g_out: torch.Tensor, x: torch.Tensor, weight: Optional[to
     lib = _lib.load()
     x, x_stride = _row_stride(x)
     g_out, g_stride = _row_stride(g_out)
-    C, dev = x.shape[-1], x.device
+    C = x.shape[-1]
     M = x.numel() // C
     g_x = torch.empty_like(x, memory_format=torch.contiguous_format)
-    g_weight = torch.empty((C,), dtype=w_dtype, device=dev) if want_weight else None
-    g_bias = torch.empty((C,), dtype=w_dtype, device=dev) if want_bias else None
+    g_weight = x.new_empty((C,), dtype=w_dtype) if want_weight else None
+    g_bias = x.new_empty((C,), dtype=w_dtype) if want_bias else None
     ws = None
     if want_weight or want_bias:
-        size = lib.nerf_layernorm_backward_workspace_bytes(M, C)
+        size = lib.nerf_layernorm_backward_workspace_bytes(M, C, code)
         if size < 0:
             _lib.check(1, "nerf_layernorm_backward_workspace_bytes")
-        ws = torch.empty((size,), dtype=torch.uint8, device=dev)
+        if size:
+            ws = x.new_empty((size,), dtype=torch.uint8)
     _enqueue(x.get_device(), "nerf_layernorm_backward", lib.nerf_layernorm_backward, g_out.data_ptr(), g_stride, x.data_ptr(),
              x_stride, code, M, C, weight.data_ptr() if weight is not None else None, _DTYPES[w_dtype], mean.data_ptr(),
              rstd.data_ptr(), g_x.data_ptr(), g_weight.data_ptr() if want_weight else None,
