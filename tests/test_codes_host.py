@@ -21,6 +21,7 @@ def test_layernorm_entries_refuse():
     assert call(P, 8, F32, -1, 8, P, P, F32, 1e-5, P, P, P, None) == ARG
     assert call(P, 8, F32, 4, 0, P, P, F32, 1e-5, P, P, P, None) == ARG
     assert call(P, 8, F32, 1 << 62, 8, P, P, F32, 1e-5, P, P, P, None) == ARG
+    assert call(P, 1 << 25, F32, 4, (1 << 24) + 1, P, P, F32, 1e-5, P, P, P, None) == ARG
     assert call(P, 7, F32, 4, 8, P, P, F32, 1e-5, P, P, P, None) == ARG and b"overlap" in lib.nerf_amd_last_error()
     for eps in (-1e-5, float("nan"), float("inf")):
         assert call(P, 8, F32, 4, 8, P, P, F32, eps, P, P, P, None) == ARG

@@ -408,6 +408,39 @@ def test_embedding_offsets_beyond_32_bits():
     assert bool((g[-1] == 3).all()) and bool((g[-2] == 5).all()) and int(torch.count_nonzero(g)) == 2 * dim
 
 
+@pytest.mark.parametrize("n,seed", [(1, 0), (700, 1), (3000, 2), (40000, 3)])
+def test_embedding_gradient_of_a_large_vocabulary(n, seed):
+    """A table of 200 MB, whose rows are cleared in part before anything is known of the ids and in part by looking them up:
+    rows of ids that occur hold their sums, every other row is exactly 0, whatever the memory held before."""
+    rows, dim, g = 100003, 1030, gen(seed)
+    for kind in ("even", "packed", "ends"):
+        ids = torch.randint(rows, (n,), generator=g)
+        if kind == "packed":                               # a run of neighbouring rows, each of them taken
+            ids = (torch.arange(n) + 70001) % rows
+        if kind == "ends":
+            ids = torch.tensor([0, rows - 1, rows - 2, 1])[torch.randint(4, (n,), generator=g)]
+        ids = ids.cuda()
+        go = randn(g, n, dim, t=BF16)
+        dirty = torch.full((rows, dim), float("nan"), device="cuda", dtype=BF16)
+        del dirty                                          # the allocator hands the same memory out again
+        got = ops.embedding_backward(go, ids, rows, 1.0)
+        taken, back = torch.unique(ids, return_inverse=True)
+        want = torch.zeros(taken.numel(), dim, dtype=torch.float64).index_add_(0, back.cpu(), go.double().cpu())
+        size = torch.zeros(taken.numel(), dim, dtype=torch.float64).index_add_(0, back.cpu(), go.double().cpu().abs())
+        t = U * (torch.bincount(back.cpu()).double()[:, None] + 3) * size
+        close(got[taken], want, t + half(BF16) * (want.abs() + t), kind)
+        got[taken] = 0
+        assert int(torch.count_nonzero(got)) == 0 and bool(got.isfinite().all()), kind
+
+
+@pytest.mark.parametrize("n,rows", [(10, 4000), (5000, 4000), (5000, 60), (50000, 4000)])
+def test_embedding_gradient_without_a_single_known_id(n, rows):
+    go = torch.randn(n, 300, device="cuda")
+    for ids in (torch.full((n,), rows, device="cuda"), torch.full((n,), -1, device="cuda"), torch.full((n,), 7, device="cuda")):
+        got = ops.embedding_backward(go, ids, rows, 1.0, padding_idx=7)
+        assert int(torch.count_nonzero(got)) == 0 and bool(got.isfinite().all())
+
+
 def test_embedding_refusals():
     table, ids = torch.zeros(10, 6, device="cuda"), torch.zeros(4, dtype=torch.int64, device="cuda")
     go = torch.zeros(4, 6, device="cuda")
@@ -484,6 +517,17 @@ def test_dropout_drops_what_it_drops():
     assert abs(int(k.sum()) - n * (1 - p)) <= 6 * (n * p * (1 - p)) ** 0.5
     other = kept(4, 0, n, p)                                # keys give masks of their own
     assert abs(int((k & other).sum()) - n * (1 - p) ** 2) <= 6 * (n * (1 - p) ** 2 * (1 - (1 - p) ** 2)) ** 0.5
+
+
+def test_dropout_of_more_elements_than_32_bits_count():
+    """2^31 + 100 elements (4.3 GB): more than one launch takes; pieces around the seam and the end against smaller calls."""
+    n = 2 ** 31 + 100
+    x = torch.ones(n, device="cuda", dtype=BF16)
+    y = ops.dropout(x, 0.25, 9, first=3)
+    for lo, hi in ((0, 5000), (2 ** 31 - 5001, 2 ** 31 + 77), (n - 100, n)):
+        assert torch.equal(y[lo:hi], ops.dropout(x[lo:hi].clone(), 0.25, 9, first=3 + lo))
+    kept_share = float((y != 0).double().mean())
+    assert abs(kept_share - 0.75) <= 6 * (0.75 * 0.25 / n) ** 0.5
 
 
 def test_dropout_key_tensor():

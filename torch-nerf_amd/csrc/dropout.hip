@@ -83,12 +83,15 @@ __global__ __launch_bounds__(256) void dropout_kernel(const T *__restrict__ x, c
 template <typename T>
 void launch(const void *x, const void *residual, int64_t n, uint32_t threshold, bool none, float scale, uint64_t key,
             const uint64_t *key_dev, int64_t first, void *out, hipStream_t stream) {
-    const int64_t pieces = (n + Row<T>::VEC - 1) / Row<T>::VEC;
-    const int64_t grid = (pieces + 255) / 256;
     auto kernel = residual ? ((first & 1) ? dropout_kernel<T, true, true> : dropout_kernel<T, false, true>)
                            : ((first & 1) ? dropout_kernel<T, true, false> : dropout_kernel<T, false, false>);
-    hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(256), 0, stream, static_cast<const T *>(x),
-                       static_cast<const T *>(residual), n, threshold, none, scale, key, key_dev, first, static_cast<T *>(out));
+    constexpr int64_t MOST = (int64_t)1 << 31;               // of one launch, whose threads are counted in 32 bits
+    for (int64_t at = 0; at < n; at += MOST) {
+        const int64_t count = n - at < MOST ? n - at : MOST, pieces = (count + Row<T>::VEC - 1) / Row<T>::VEC;
+        hipLaunchKernelGGL(kernel, dim3((unsigned)((pieces + 255) / 256)), dim3(256), 0, stream, static_cast<const T *>(x) + at,
+                           residual ? static_cast<const T *>(residual) + at : nullptr, count, threshold, none, scale, key, key_dev,
+                           first + at, static_cast<T *>(out) + at);
+    }
 }
 
 }  // namespace

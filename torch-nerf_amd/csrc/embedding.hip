@@ -776,9 +776,14 @@ void launch_forward(const void *table, int64_t rows, int64_t row_stride, int64_t
     const int64_t per = packed ? 1024 / pieces : 1;
     const unsigned threads = packed ? (unsigned)((per * pieces + WAVE - 1) / WAVE * WAVE) : 256;
     auto kernel = dim < Row<T>::VEC ? embedding_kernel<T, true, 1> : packed ? embedding_kernel<T, false, 1> : embedding_kernel<T, false, 4>;
-    hipLaunchKernelGGL(kernel, dim3((unsigned)((n + per - 1) / per)), dim3(threads), 0, stream, static_cast<const T *>(table),
-                       rows, row_stride, (int)dim, ids, wide, n, scale, (int)pieces,
-                       (uint32_t)(((1 << 20) + pieces - 1) / pieces), (int)per, static_cast<T *>(out));
+    const int64_t most = ((int64_t)1 << 31) / threads * per;                // rows of a launch, whose threads are counted in 32 bits
+    for (int64_t at = 0; at < n; at += most) {
+        const int64_t count = n - at < most ? n - at : most;
+        hipLaunchKernelGGL(kernel, dim3((unsigned)((count + per - 1) / per)), dim3(threads), 0, stream,
+                           static_cast<const T *>(table), rows, row_stride, (int)dim,
+                           static_cast<const char *>(ids) + at * (wide ? 8 : 4), wide, count, scale, (int)pieces,
+                           (uint32_t)(((1 << 20) + pieces - 1) / pieces), (int)per, static_cast<T *>(out) + at * dim);
+    }
 }
 
 // Unconditional clearing of `count` values, shared out to workgroups of SORT_THREADS.

@@ -70,7 +70,7 @@ template <typename T, int TPR, int NV, bool WIDE, bool TINY>
 __global__ __launch_bounds__(WIDE ? 1024 : 256) void layernorm_kernel(const T *__restrict__ x, int64_t x_stride, int64_t M, int C,
                                                           const void *__restrict__ weight, const void *__restrict__ bias,
                                                           int w_f32, float eps, T *__restrict__ y,
-                                                          float *__restrict__ mean, float *__restrict__ rstd, int waves, int per) {
+                                                          float *__restrict__ mean, float *__restrict__ rstd, int waves, int64_t per) {
     constexpr int VEC = Row<T>::VEC;
     constexpr bool HOIST = NV * VEC <= 8;                     // the weights stay in registers from row to row
     __shared__ float red[WIDE ? 2 * MAX_WAVES : 1];
@@ -293,15 +293,12 @@ __global__ __launch_bounds__(1024) void layernorm_bwd_kernel(const T *__restrict
     }
     if (!g_weight && !g_bias) return;
     // one workgroup alone has the gradients themselves
-    auto put = [&](int c, float w_sum, float b_sum) {
-        if (gridDim.x > 1) {
-            float *dst = partial + (int64_t)blockIdx.x * 2 * C;
-            dst[c] = w_sum;
-            dst[C + c] = b_sum;
-        } else {
-            if (g_weight) store_column<T>(g_weight, w_f32, c, w_sum);
-            if (g_bias) store_column<T>(g_bias, w_f32, c, b_sum);
-        }
+    auto put = [&](int c, float sum, bool bias) {
+        void *out = bias ? g_bias : g_weight;
+        if (gridDim.x > 1)
+            partial[((int64_t)blockIdx.x * 2 + (bias ? 1 : 0)) * C + c] = sum;
+        else if (out)
+            store_column<T>(out, w_f32, c, sum);
     };
     // lane groups of a wavefront first, then the groups of the workgroup through LDS, in order
 #pragma unroll
@@ -319,33 +316,32 @@ __global__ __launch_bounds__(1024) void layernorm_bwd_kernel(const T *__restrict
             const nerf::Place<T, TINY> at((i * width + lane) * VEC, C);
 #pragma unroll
             for (int j = 0; j < VEC; ++j)
-                if (at.own(j)) put(at.at + j, gw[i][j], gb[i][j]);
+                if (at.own(j)) { put(at.at + j, gw[i][j], false); put(at.at + j, gb[i][j], true); }
         }
         return;
     }
-    // [group][NV * VEC][gw, gb][width]
-    const int mine = threadIdx.x / lanes, size = NV * VEC * 2 * width;
-    if ((int)threadIdx.x - mine * lanes < width) {
+    // gw, then gb: [group][NV * VEC][width]
+    const int mine = threadIdx.x / lanes, size = NV * VEC * width;
+    const bool has = (int)threadIdx.x - mine * lanes < width;
+    auto join = [&](const float (&v)[NV][VEC], bool bias) {
+        __syncthreads();
+        if (has) {
 #pragma unroll
-        for (int i = 0; i < NV; ++i)
+            for (int i = 0; i < NV; ++i)
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) {
-                float *c = cols + mine * size + (i * VEC + j) * 2 * width + lane;
-                c[0] = gw[i][j];
-                c[width] = gb[i][j];
-            }
-    }
-    __syncthreads();
-    for (int k = threadIdx.x; k < width * NV * VEC; k += blockDim.x) {
-        const int l = k % width, ij = k / width, j = ij % VEC;
-        const nerf::Place<T, TINY> at(((ij / VEC) * width + l) * VEC, C);
-        float w_sum = 0.0f, b_sum = 0.0f;
-        for (int g = 0; g < groups; ++g) {
-            w_sum += cols[g * size + ij * 2 * width + l];
-            b_sum += cols[g * size + ij * 2 * width + width + l];
+                for (int j = 0; j < VEC; ++j) cols[mine * size + (i * VEC + j) * width + lane] = v[i][j];
         }
-        if (at.own(j)) put(at.at + j, w_sum, b_sum);
-    }
+        __syncthreads();
+        for (int k = threadIdx.x; k < size; k += blockDim.x) {
+            const int l = k % width, ij = k / width, j = ij % VEC;
+            const nerf::Place<T, TINY> at(((ij / VEC) * width + l) * VEC, C);
+            float sum = 0.0f;
+            for (int g = 0; g < groups; ++g) sum += cols[g * size + k];
+            if (at.own(j)) put(at.at + j, sum, bias);
+        }
+    };
+    join(gw, false);
+    join(gb, true);
 }
 
 // out[c] = sum over the G partial rows of column c: 16 columns x 64 slices of the partial rows per workgroup
@@ -488,11 +484,13 @@ void launch_forward(const void *x, int64_t x_stride, int64_t M, int64_t C, const
     // Every workgroup takes its rows once, in the order of the addresses: 1 GB of fp32 rows of 256 at 6.2 TB/s, where 2048
     // workgroups that stride over the rows reach 5.2.  Short 16-bit rows are too little work for that (4.8 TB/s: the
     // weights come first): 4 of them one after another, 5.8 TB/s.
-    auto run = [&](auto kernel, int64_t rows, int waves, int per) {
+    auto run = [&](auto kernel, int64_t rows, int waves, int64_t in_turn) {
         const int64_t steps = (M + rows - 1) / rows;
-        if (steps < 4 * 2048) per = 1;
+        const int threads = waves ? waves * WAVE : 256;
+        int64_t per = steps < 4 * 2048 ? 1 : in_turn;
+        while ((steps + per - 1) / per * threads > (int64_t)1 << 31) per *= 2;       // a launch's threads are counted in 32 bits
         const int64_t grid = (steps + per - 1) / per;
-        hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(waves ? waves * WAVE : 256), 0, stream, xt, x_stride, M, (int)C,
+        hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(threads), 0, stream, xt, x_stride, M, (int)C,
                            weight, bias, w_f32, eps, yt, mean, rstd, waves, per);
     };
 #define LN_RUN run(layernorm_kernel<T, TPR, NV, WIDE, TINY>, WIDE ? 1 : 256 / TPR, WIDE ? (int)((C + NV * VEC * WAVE - 1) / (NV * VEC * WAVE)) : 0, NV == 1 && VEC == 8 && !WIDE ? 4 : 1)
@@ -568,7 +566,7 @@ void launch_backward(const void *g_out, int64_t g_stride, const void *x, int64_t
     } else if (M > 0) {
         // LDS: the column sums of every group of lanes that has one, where there is more than one group
         auto run = [&](auto kernel, int lanes, int values) {
-            const int lds = lanes < walk.threads ? (lanes < WAVE ? walk.threads / WAVE : walk.threads / lanes) * lanes * values * 8 : 0;
+            const int lds = lanes < walk.threads ? (lanes < WAVE ? walk.threads / WAVE : walk.threads / lanes) * lanes * values * 4 : 0;
             hipLaunchKernelGGL(kernel, dim3((unsigned)walk.groups), dim3(walk.threads), lds, stream, gt, g_stride, xt, x_stride, M,
                                (int)C, weight, w_f32, mean, rstd, gx, partial, g_weight, g_bias, walk.waves,
                                walk.per);
@@ -591,7 +589,7 @@ void launch_backward(const void *g_out, int64_t g_stride, const void *x, int64_t
     }
 }
 
-bool sizes_ok(int64_t M, int64_t C) { return M >= 0 && C >= 1 && C <= (int64_t)1 << 30 && M <= INT64_MAX / 8 / C; }
+bool sizes_ok(int64_t M, int64_t C) { return M >= 0 && C >= 1 && C <= (int64_t)1 << 24 && M <= INT64_MAX / 8 / C; }
 
 }  // namespace
 
