@@ -6,6 +6,11 @@
 // and any sharding of the batch see the same one, and a second evaluation costs less than a byte per element would.
 //   y = keep ? x / (1 - p) : 0        (+ residual)
 // A dropped element is 0 whatever x holds there (an infinity or NaN in a dropped place does not pass).
+//
+// Bound by HBM: 786432 x 256 bf16 in 130 us, 6.2 TB/s; 16383 x 2047 bf16 with a residual in 31 us, 6.4 TB/s.  The generator
+// is not far behind: two elements take six quarter-rate multiplications (24 x 16 of about 700 cycles a piece of 8), 110 us
+// of this case if nothing else did anything.  As 64-bit arithmetic with a 64-bit comparison the kernel took 162 us; as a
+// grid that strides over the array, 187.
 #include <math.h>
 
 #include "rows.h"

@@ -5,7 +5,13 @@
 //
 // A row stays in registers between its one read and its one write: TPR lanes hold it as NV 16-byte pieces each.  The
 // variance is taken about the mean (a second sum over the registers), so a large offset costs no digits.  Statistics and
-// sums are fp32.  Rows of up to 64 lanes need no barrier; a longer row takes a workgroup.
+// sums are fp32.  Rows of up to 64 lanes need no barrier; a longer row takes several wavefronts.
+//
+// Bound by HBM.  Forward 262144 x 256 fp32: 90 us, 6.0 TB/s read + written (a copy of that size: 5.4); 16384 x 2048 bf16
+// 26 us (5.1); 1 row of 4096: 2.6 us.  Backward 786432 x 256 fp32: 453 + 12 us for the columns, 5.2 TB/s; 8192 x 4096 bf16:
+// 41 + 5 us, 4.4 TB/s.  Where it is not: rows of 8193..16384 values (a workgroup holds one row, in lockstep: 8192 x 4096
+// values as 2048 x 16384 bf16 take 79 us backward instead of 41), and rows of fewer than 8 16-bit or 4 fp32 values (value by
+// value).
 #include "rows.h"
 
 namespace {

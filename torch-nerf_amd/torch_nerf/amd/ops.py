@@ -688,9 +688,9 @@ def _row_stride(t: torch.Tensor):
 
 
 def _enqueue(device_index: int, what: str, fn, *args) -> None:
-    """One call of the C ABI on the current stream of that GPU.  (The stream's raw handle: a Stream object around it takes
-    2.6 us, as much as the launch.)"""
-    if device_index == torch.cuda.current_device():
+    """One call of the C ABI on the current stream of that GPU.  (Its raw handle: a Stream object around it takes 2.6 us, as
+    much as the launch.)"""
+    if device_index == torch._C._cuda_getDevice():
         rc = fn(*args, torch._C._cuda_getCurrentRawStream(device_index))
     else:
         with torch.cuda.device(device_index):
