@@ -281,7 +281,8 @@ EMB = [(1, 1, 1), (1, 5, 3), (7, 3, 16), (64, 10, 5), (300, 100, 48), (513, 1, 3
        (70000, 37, 4),
        (1024, 50, 6), (1025, 50, 6), (32768, 3000, 7), (32769, 3000, 7), (3000, 40000, 1030), (50, 30000, 700),
        (40000, 100000, 264),
-       (65536, 255, 33), (65537, 64, 33), (65537, 65, 12), (90000, 128, 6), (90000, 129, 6), (700, 255, 2100)]
+       (65536, 255, 33), (65537, 64, 33), (65537, 65, 12), (90000, 128, 6), (90000, 129, 6), (700, 255, 2100),
+       (70000, 3000000, 2), (5000, 2000000, 3), (50000, 300, 1100), (300000, 1000, 5)]
 
 
 def check_embedding_backward(go, ids, rows, scale, pad, what=""):

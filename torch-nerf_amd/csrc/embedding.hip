@@ -82,12 +82,12 @@ __global__ __launch_bounds__(1024) void embedding_zero_kernel(T *__restrict__ g_
 
 // ------------------------------------------------------------------------------------------------ sort
 // Stable least-significant-digit radix sort of (key, position), 32 bits each.  Keys are the ids; ids that give no gradient
-// take the key `rows`, behind all others.  A digit has at most 9 bits.
+// take the key `rows`, behind all others.  A digit has at most 10 bits (a thread a digit).
 //
 // One tile is 1024 threads x ITEMS pairs, a wavefront holding 64 consecutive pairs per step, so that the order inside a
 // digit is (wavefront, step, lane).  `rank` finds a pair's place among the equal digits before it: the lanes that share
 // its digit by one ballot per bit, plus the count its wavefront kept so far.
-constexpr int SORT_THREADS = 1024, SORT_WAVES = SORT_THREADS / WAVE, MAX_DIGIT_BITS = 9, MAX_BINS = 1 << MAX_DIGIT_BITS;
+constexpr int SORT_THREADS = 1024, SORT_WAVES = SORT_THREADS / WAVE, MAX_DIGIT_BITS = 10, MAX_BINS = 1 << MAX_DIGIT_BITS;
 constexpr int TILE_ITEMS = 4, TILE = SORT_THREADS * TILE_ITEMS;            // of a pass over many tiles
 constexpr int MERGE_TILES = 32, MERGE_MOST = MERGE_TILES * SORT_THREADS;   // sorted tiles of 1024, merged
 
@@ -487,45 +487,55 @@ __global__ __launch_bounds__(SUM_THREADS) void embedding_sum_kernel(const T *__r
     }
 }
 
-// One workgroup a span and 256 columns, 4 a lane; it has work where an id begins in the span and goes on behind it: the
-// first partial row and those of the spans that follow, one wavefront every fourth of them.
+// One workgroup a span and up to 256 columns; it has work where an id begins in the span and goes on behind it: the first
+// partial row and those of the spans that follow, 4 columns a lane, 2^shift lanes a row, the lane groups every so many rows
+// and then in order.
+constexpr int JOIN_THREADS = 256;        // (1024: 15 us more where every second span has work, 16384 x 1024)
+
 template <typename T, bool TINY>
-__global__ __launch_bounds__(256) void embedding_join_kernel(const uint32_t *__restrict__ keys, int64_t n, int dim,
-                                                             float scale, int64_t span, const float *__restrict__ partial,
-                                                             const uint32_t *__restrict__ goes_on, T *__restrict__ g_table) {
-    __shared__ float part[4][256];
+__global__ __launch_bounds__(JOIN_THREADS) void embedding_join_kernel(const uint32_t *__restrict__ keys, int64_t n, int dim,
+                                                                      float scale, int64_t span, int shift,
+                                                                      const float *__restrict__ partial,
+                                                                      const uint32_t *__restrict__ goes_on,
+                                                                      T *__restrict__ g_table) {
+    __shared__ float part[JOIN_THREADS * 4];
     const int64_t c = blockIdx.x, spans = (n + span - 1) / span;
     if (!goes_on[c]) return;
-    const int lane = threadIdx.x & 63, s = threadIdx.x >> 6;
+    const int lane64 = threadIdx.x & (WAVE - 1);
     const uint32_t key = keys[(c + 1) * span];
     // the last span that begins inside of the id: 64 spans a step, the steps growing by 64 while all of them do
     int64_t last = c + 1, step = 1;
     for (bool grow = true; step > 0;) {
-        const int64_t probe = last + (lane + 1) * step;
+        const int64_t probe = last + (lane64 + 1) * step;
         const uint64_t in = __ballot(probe < spans && keys[probe * span] == key);
         const int more = in == ~0ull ? 64 : __ffsll((long long)~in) - 1;
         last += more * step;
         if (more < 64) grow = false;
         step = grow ? step * 64 : step / 64;
     }
-    for (int base = blockIdx.y * 256; base < dim; base += gridDim.y * 256) {
-        const nerf::Place<float, TINY> at(base + lane * 4, dim);
-        float sum[4] = {};
-        auto add = [&](int64_t k, int which) {
-            const Row<float> r = nerf::load_piece<TINY>(partial + (k * 2 + which) * dim, at);
+    const int group = threadIdx.x >> shift, groups = JOIN_THREADS >> shift, lane = threadIdx.x & ((1 << shift) - 1), width = 4 << shift;
+    for (int column = blockIdx.y * width; column < dim; column += gridDim.y * width) {
+        const nerf::Place<float, TINY> at(column + lane * 4, dim);
+        if (at.live()) {
+            float sum[4] = {};
+            auto add = [&](int64_t k, int which) {
+                const Row<float> r = nerf::load_piece<TINY>(partial + (k * 2 + which) * dim, at);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) sum[j] += r.v[j];
-        };
-        if (s == 0) add(c, 1);
-#pragma unroll 4
-        for (int64_t k = c + 1 + s; k <= last; k += 4) add(k, 0);
+                for (int j = 0; j < 4; ++j) sum[j] += r.v[j];
+            };
+            if (group == 0) add(c, 1);
+#pragma unroll 8
+            for (int64_t k = c + 1 + group; k <= last; k += groups) add(k, 0);
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (at.own(j)) part[s][at.at + j - base] = sum[j];
+            for (int j = 0; j < 4; ++j)
+                if (at.own(j)) part[group * width + at.at + j - column] = sum[j];
+        }
         __syncthreads();
-        const int col = threadIdx.x;
-        if (base + col < dim)
-            g_table[(int64_t)key * dim + base + col] = (T)((part[0][col] + part[1][col] + part[2][col] + part[3][col]) * scale);
+        for (int col = threadIdx.x; col < width && column + col < dim; col += JOIN_THREADS) {
+            float s = 0.0f;
+            for (int g = 0; g < groups; ++g) s += part[g * width + col];
+            g_table[(int64_t)key * dim + column + col] = (T)(s * scale);
+        }
         __syncthreads();
     }
 }
@@ -879,10 +889,12 @@ int launch_backward(const void *g_out, int dtype, int64_t n, int64_t dim, const 
                        static_cast<const T *>(g_out), n, (int)dim, keys, order, (uint32_t)rows, scale, p.chunk, p.shift, gt,
                        partial, words(p.goes_on), p.spans, cleared, (int)clear_rows);
     if (p.spans > 1) {
-        int64_t gy = (dim + 255) / 256;
+        const int shift = lane_shift((dim + 3) / 4) < 6 ? lane_shift((dim + 3) / 4) : 6;
+        const int64_t gy = (dim + 255) / 256;
         auto join = dim < Row<float>::VEC ? embedding_join_kernel<T, true> : embedding_join_kernel<T, false>;
-        hipLaunchKernelGGL(join, dim3((unsigned)(p.spans - 1), (unsigned)(gy < 16 ? gy : 16)), dim3(256), 0, stream, keys, n,
-                           (int)dim, scale, (int64_t)p.chunk * (SUM_THREADS >> p.shift), partial, words(p.goes_on), gt);
+        hipLaunchKernelGGL(join, dim3((unsigned)(p.spans - 1), (unsigned)(gy < 16 ? gy : 16)), dim3(JOIN_THREADS), 0, stream,
+                           keys, n, (int)dim, scale, (int64_t)p.chunk * (SUM_THREADS >> p.shift), shift, partial,
+                           words(p.goes_on), gt);
     }
     return NERF_OK;
 }
