@@ -430,9 +430,9 @@ __global__ __launch_bounds__(SUM_THREADS) void embedding_sum_kernel(const T *__r
                     if (at.own(j)) dst[j] = sum[j];
             }
         };
-        for (int64_t i = lo; i < hi; i += AHEAD) {
-            // the rows of this step are on their way while the ids of the next one are read (rows of ids that give no
-            // gradient as well: their sum goes nowhere)
+        // (sorted: where the first id gives no gradient, none of the chunk does; one at the chunk's end is read for nothing)
+        for (int64_t i = first < rows ? lo : hi; i < hi; i += AHEAD) {
+            // the rows of this step are on their way while the ids of the next one are read
             Row<T> r[AHEAD];
             uint32_t now[AHEAD];
 #pragma unroll
@@ -816,9 +816,8 @@ struct Clear {
     }
 };
 
-// What the chip clears while a sorting launch of some 10 us lasts (65 us a gradient of 16384 x 1024 bf16 into 131072 rows;
-// 70 with 40 MB, 80 with none), and the shortest row that the summing launch clears (a
-// shorter one is less than 32 pieces: looking it up costs more than the store).
+// What the chip clears while a sorting launch of some 10 us lasts (16384 x 1024 bf16 into 131072 rows: 65 us; 70 with 40 MB, 80
+// with none), and the shortest row that the summing launch clears (one of fewer than 32 pieces is stored sooner than looked up).
 constexpr int64_t CLEAR_BESIDE_SORT = (int64_t)60 << 20, CLEAR_ABSENT_BYTES = 512;
 
 template <typename T>
