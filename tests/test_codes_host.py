@@ -106,3 +106,17 @@ def test_modules_share_their_state_with_torch():
     assert list(layers.LayerNorm(5, affine=False).parameters()) == [] and layers.LayerNorm(5, bias=False).bias is None
     x = torch.randn(3)
     assert layers.Dropout(0.5).eval()(x) is x and layers.Dropout(0.0)(x) is x
+
+
+def test_functions_and_modules_refuse_before_the_backward_pass_would():
+    """What training would refuse, or refuse only in the backward pass, is refused by the forward call and in evaluation."""
+    table, ids = torch.zeros(4, 8, requires_grad=True), torch.zeros(4, dtype=torch.int64)
+    for pad in (-1, 4):
+        with pytest.raises(ValueError, match="padding_idx"):
+            ops.EmbeddingFunction.apply(table, ids, 1.0, pad)
+    x = torch.zeros(4, 8)
+    drop = layers.Dropout(0.5).eval()
+    for r in (x[:1], x.double(), x[0], 1.0):
+        with pytest.raises(ValueError, match="residual"):
+            drop(x, r)
+    assert torch.equal(drop(x, x + 1), x + 1)

@@ -627,6 +627,24 @@ def test_functions_give_gradients_only_where_asked():
     assert torch.equal(shared.grad, r + ops.dropout(r, 0.5, 3))
 
 
+def test_layernorm_bias_alone_keeps_its_digits():
+    """16-bit rows with an fp32 bias and no weight: the bias's gradient is an fp32 sum (99 additions at most along a term's
+    way, below 100 U of the magnitudes), not one that was rounded to 16 bits first."""
+    g = gen(21)
+    for t in (BF16, F16):
+        x, b, up = randn(g, 99, 40, t=t), randn(g, 40), randn(g, 99, 40, t=t)
+        bias = b.clone().requires_grad_(True)
+        ops.LayerNormFunction.apply(x, None, bias, 1e-5).backward(up)
+        close(bias.grad, up.double().sum(0), 100 * U * up.double().abs().sum(0))
+        mu, r = ops.layernorm(x, None, b, want_stats=True)[1:]
+        assert ops.layernorm_backward(up, x, None, mu, r)[2].dtype == t
+        w = randn(g, 40, t=t)
+        with pytest.raises(ValueError, match="bias_dtype"):
+            ops.layernorm_backward(up, x, w, mu, r, bias_dtype=F32)
+        with pytest.raises(ValueError, match="bias_dtype"):
+            ops.layernorm_backward(up, x, None, mu, r, bias_dtype=torch.float64)
+
+
 def test_modules_in_a_conditioned_network():
     """A code per view, normalised and dropped out, behind NeRF's view direction, trained with the network under FusedAdam:
     forward and all gradients against torch in 64 bits, and the whole step without a host synchronisation in between."""
@@ -718,6 +736,38 @@ def test_captured_and_replayed():
         for _, _, step, res in graphs:
             assert all(torch.equal(a, b) for a, b in zip(step(), res))
         torch.cuda.synchronize()
+
+
+def test_modules_captured_with_their_backward_pass():
+    """The modules' forward and autograd's backward pass in one graph (no eager graph of the parameters lives meanwhile),
+    replayed with new inputs and keys, every replay against the eager result."""
+    torch.manual_seed(22)
+    codes, norm = layers.Embedding(50, 24, scale=0.5, padding_idx=0).cuda(), layers.LayerNorm(24).cuda()
+    drop = layers.Dropout(0.3)
+    params = [*codes.parameters(), *norm.parameters()]
+    ids, up = torch.randint(50, (5000,), device="cuda"), torch.randn(5000, 24, device="cuda")
+    key = torch.tensor([7], device="cuda")
+
+    def step():
+        out = drop(norm(codes(ids)), key=key)
+        return [out.detach(), *torch.autograd.grad(out, params, up)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        res = step()
+    for turn in range(4):
+        ids.copy_(torch.randint(50, ids.shape, device="cuda"))
+        up.normal_()
+        key += 1
+        graph.replay()
+        want = step()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(want, res))
 
 
 def test_dropout_module_refuses_a_capture_without_a_key():

@@ -3,7 +3,8 @@
 A latent code per view (or per object, per frame) is looked up by ``Embedding``, normalised by ``LayerNorm``, regularised by
 ``Dropout`` and concatenated to the encoded view direction; NeRF's kernels return the gradient of that input, so the codes
 train with the networks, also under ``optim.FusedAdam``.  Parameters are named and initialised like torch.nn's modules of the
-same names, so their state_dicts are interchangeable.  There is no CPU fallback: the modules raise for tensors off the GPU.
+same names, so their state_dicts are interchangeable.  There is no CPU fallback: the modules raise for tensors off the GPU
+(a Dropout that drops nothing launches nothing, and takes any).
 """
 from typing import Optional
 
@@ -53,7 +54,9 @@ class LayerNorm(nn.Module):
 class Dropout(nn.Module):
     """Counter-based dropout.  The n-th call in training mode uses key(seed, n): give every module a seed of its own, and
     the same one on every rank (a rank passes the flat index of its first element as `first`).  Inside a graph capture the
-    count would be frozen into the graph: pass a key tensor there."""
+    count would be frozen into the graph: pass a key tensor there.  A forward that is run again for its gradient (activation
+    checkpointing) would count twice and draw another mask: pass a key there, too.  The count (`calls`) is not part of the
+    state_dict, whose keys are torch.nn.Dropout's (none): a resumed run sets it."""
 
     def __init__(self, p: float = 0.5, seed: int = 0):
         super().__init__()
@@ -63,7 +66,9 @@ class Dropout(nn.Module):
 
     def forward(self, x: torch.Tensor, residual: Optional[torch.Tensor] = None, first: int = 0, key=None) -> torch.Tensor:
         if not self.training or self.p == 0.0:
-            return x if residual is None else x + residual
+            if residual is None:
+                return x
+            return x + ops._like(residual, "residual", x, "x")
         if key is None:
             if x.is_cuda and torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("Dropout inside a graph capture needs a key tensor: its own key would never change")

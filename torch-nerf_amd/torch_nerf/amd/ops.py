@@ -760,6 +760,8 @@ class EmbeddingFunction(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, table, ids, scale=1.0, padding_idx=None):
+        if padding_idx is not None and not 0 <= padding_idx < table.shape[0]:
+            raise ValueError(f"padding_idx {padding_idx} is not one of {table.shape[0]} rows")
         ctx.num_rows, ctx.scale, ctx.padding_idx = table.shape[0], float(scale), padding_idx
         ctx.save_for_backward(ids)
         return embedding(table, ids, scale)
@@ -810,13 +812,19 @@ def layernorm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opti
 
 
 def layernorm_backward(g_out: torch.Tensor, x: torch.Tensor, weight: Optional[torch.Tensor], mean: torch.Tensor,
-                       rstd: torch.Tensor, want_weight: bool = True, want_bias: bool = True):
+                       rstd: torch.Tensor, want_weight: bool = True, want_bias: bool = True,
+                       bias_dtype: Optional[torch.dtype] = None):
     """-> (g_x, g_weight | None, g_bias | None) of `layernorm`.  mean, rstd: what its want_stats returned.  The gradients
-    of weight and bias are of weight's type (x's where there is none), summed over the rows in fp32 in a fixed order."""
+    of weight and bias are of weight's type (without a weight: bias_dtype, x's or float32, x's if not given), summed over
+    the rows in fp32 in a fixed order."""
     code = _rows(x, "x")
     if x.ndim < 1 or x.shape[-1] < 1:
         raise ValueError(f"x: expected (..., C) with C >= 1, got {tuple(x.shape)}")
     weight, _, w_dtype = _norm_weights(x, weight, None)
+    if bias_dtype is not None and bias_dtype != w_dtype:
+        if weight is not None or bias_dtype != torch.float32:
+            raise ValueError(f"bias_dtype: expected {w_dtype}{'' if weight is not None else ' or float32'}, got {bias_dtype}")
+        w_dtype = bias_dtype
     mean = _like(mean, "mean", x, "x", shape=x.shape[:-1], dtype=torch.float32)
     rstd = _like(rstd, "rstd", x, "x", shape=x.shape[:-1], dtype=torch.float32)
     if g_out.shape != x.shape or g_out.dtype != x.dtype or g_out.device != x.device:
@@ -859,9 +867,7 @@ class LayerNormFunction(torch.autograd.Function):
     def backward(ctx, g_out):
         x, weight, mean, rstd = ctx.saved_tensors
         g_x, g_w, g_b = layernorm_backward(g_out, x, weight, mean, rstd, want_weight=any(ctx.needs_input_grad[1:2]),
-                                           want_bias=any(ctx.needs_input_grad[2:3]))
-        if g_b is not None and g_b.dtype != ctx.bias_dtype:      # an fp32 bias without a weight over 16-bit rows
-            g_b = g_b.to(ctx.bias_dtype)
+                                           want_bias=any(ctx.needs_input_grad[2:3]), bias_dtype=ctx.bias_dtype)
         return g_x, g_w, g_b, None
 
 
