@@ -196,6 +196,71 @@ def test_layernorm_keeps_digits_under_a_large_offset():
     close(r, torch.full((4,), 1e-5).double().rsqrt(), torch.full((4,), 1e3 * U))
 
 
+def check_norm_offset(x, w, b, eps=1e-5, what=""):
+    """y, mean and rstd with bounds that an offset common to a row's values does not widen, but for the one rounding of a
+    mean that is stored as fp32.
+
+    With u = x - x0 (rounded: U |u|), k additions on a term's way: the first mean m is off by at most delta =
+    U |mu| + (k + 3) U mean|u|.  d = x - m is off by U |d|, |d| <= D = |x - mu| + delta; e = mean(d) by (k + 3) U A, A = mean D.
+    So the numerator x - m - e is off by U D + (k + 5) U A (the last two: the product e r).  The variance mean(d^2) - e^2 is
+    off by (k + 6) U (V + delta^2) + 2 (delta + (k + 3) U A) (k + 3) U A + U delta^2, where V is the exact one; 1 / sqrt
+    takes half of that relative to V + eps (0.75 with the higher orders, below 0.2) and 4 roundings."""
+    y, mu, r = ops.layernorm(x, w, b, eps, want_stats=True)
+    xd, C = x.double(), x.shape[-1]
+    k = adds(C)
+    m64 = xd.mean(-1, keepdim=True)
+    dev = (xd - m64).abs()
+    V = (dev * dev).mean(-1, keepdim=True)
+    r64 = 1.0 / torch.sqrt(V + eps)
+    delta = U * m64.abs() + (k + 3) * U * (xd - xd[..., :1]).abs().mean(-1, keepdim=True)
+    D = dev + delta
+    A = D.mean(-1, keepdim=True)
+    t_e = (k + 3) * U * A
+    t_V = ((k + 6) * U * (V + delta ** 2) + 2 * (delta + t_e) * t_e + U * delta ** 2) / (V + eps)
+    assert float(t_V.max()) < 0.2, what
+    t_r = r64 * (0.75 * t_V + 4 * U)
+    h = (xd - m64) * r64
+    wd, bd = w.double(), b.double()
+    want = h * wd + bd
+    t_y = wd.abs() * (r64 * (U * D + (k + 5) * U * A) + dev * t_r + 3 * U * h.abs()) + 2 * U * ((h * wd).abs() + bd.abs())
+    close(mu, m64[..., 0], (t_e + 2 * U * (m64.abs() + delta))[..., 0], what + " mean")
+    close(r, r64[..., 0], t_r[..., 0], what + " rstd")
+    close(y, want, t_y + half(x.dtype) * (want.abs() + t_y) + step0(x.dtype), what + " y")
+
+
+@pytest.mark.parametrize("t", DTYPES)
+@pytest.mark.parametrize("C", [1, 3, 48, 255, 300, 600, 2047, 3000, 8191, 16000, 20011])
+def test_layernorm_of_rows_with_an_offset(t, C):
+    """Constant rows whose sums are inexact, and small deviations on a large offset (in 16 bits: what is left of them), in
+    rows of one lane up to rows of several sweeps, few and many of them; and a first value far from all others."""
+    g = gen(C)
+    w, b = randn(g, C, t=t), randn(g, C, t=t)
+    for M in (3, 1100 if C <= 4096 else 40):
+        for offset, size in ((3333.3, 0.0), (1e4, 0.0), (-6e4, 0.0), (1e4, 0.01), (3e4, 1.0), (-777.7, 30.0)):
+            x = randn(g, M, C, t=t, scale=size, shift=offset)
+            check_norm_offset(x, w, b, what=f"{M}x{C} {t} {offset} {size}")
+        x = randn(g, M, C, t=t)
+        x[:, 0] = 1000.0
+        check_norm_offset(x, w, b, what=f"{M}x{C} {t} first value")
+    same = torch.full((5, C), 3333.3, device="cuda").to(t)
+    y, mu, r = ops.layernorm(same, None, b, want_stats=True)
+    assert torch.equal(y, b.expand(5, C)) and torch.equal(mu, same[:, 0].float())      # constant rows: 0 to the last bit
+
+
+@pytest.mark.parametrize("t", [F32, BF16])
+@pytest.mark.parametrize("C", [3, 70, 3000, 20011])
+def test_layernorm_of_the_lowest_value(t, C):
+    """A row with its type's lowest value in it: the variance is beyond fp32, rstd 0 and the row its bias, as without an
+    offset's care; rows beside it are untouched."""
+    g = gen(C)
+    x, b = randn(g, 4, C, t=t), randn(g, C, t=t)
+    clean = ops.layernorm(x, None, b)
+    x[1, 0] = x[2, C - 1] = torch.finfo(t).min
+    y, mu, r = ops.layernorm(x, None, b, want_stats=True)
+    assert bool((r[1:3] == 0).all()) and torch.equal(y[1:3], b.expand(2, C)) and bool(mu.isfinite().all())
+    assert torch.equal(y[0], clean[0]) and torch.equal(y[3], clean[3])
+
+
 def test_layernorm_infinities_and_nans_stay_in_their_rows():
     g = gen(3)
     x = randn(g, 9, 70)

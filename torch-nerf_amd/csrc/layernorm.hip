@@ -3,9 +3,13 @@
 //   y = (x - mu) r w + b,   mu = mean(x),  r = 1 / sqrt(mean((x - mu)^2) + eps)
 //   gx = r (q - mean(q) - h mean(q h)),  q = g w, h = (x - mu) r;   gw = sum_rows g h,   gb = sum_rows g
 //
-// A row stays in registers between its one read and its one write: TPR lanes hold it as NV 16-byte pieces each.  The
-// variance is taken about the mean (a second sum over the registers), so a large offset costs no digits.  Statistics and
-// sums are fp32.  Rows of up to 64 lanes need no barrier; a longer row takes several wavefronts.
+// A row stays in registers between its one read and its one write: TPR lanes hold it as NV 16-byte pieces each.  Statistics
+// and sums are fp32, and an offset of the row costs no digits: a plain sum of x would be off by some roundings of the
+// offset's size, which may be larger than the deviations.  So the first sum is of x - x0, x0 the row's first value, which
+// gives m, a mean to within about a rounding, and the second sums are of d = x - m and of d^2; with e = mean(d)
+//   mu = m + e,   var = mean(d^2) - e^2,   (x - mu) r = d r - e r
+// are off by roundings of the deviations' size.  (mu itself is stored as fp32, and that is what the backward pass takes.)
+// Rows of up to 64 lanes need no barrier; a longer row takes several wavefronts.
 //
 // Bound by HBM.  Forward 262144 x 256 fp32: 90 us, 6.0 TB/s read + written (a copy of that size: 5.4); 16384 x 2048 bf16
 // 26 us (5.1); 1 row of 4096: 2.6 us.  Backward 786432 x 256 fp32: 453 + 12 us for the columns, 5.2 TB/s; 8192 x 4096 bf16:
@@ -72,6 +76,22 @@ __device__ __forceinline__ void forget(Row<T> &p) {
     __builtin_memcpy(&p, u, 16);
 }
 
+// x0.  0 in place of a value so large that a sum of C differences from it could overflow where the values' own does not.
+template <typename T>
+__device__ __forceinline__ float first_value(const T *row) {
+    const float v = (float)row[0];
+    return fabsf(v) < 1e30f ? v : 0.0f;
+}
+
+// From the sums of d and of d^2, d = x - m with a first mean m: e, the mean of d, and r.
+struct Moments {
+    float e, r;
+    __device__ __forceinline__ Moments(const float (&sums)[2], float inv_c, float eps) : e(sums[0] * inv_c) {
+        const float var = fmaf(-e, e, sums[1] * inv_c);
+        r = 1.0f / sqrtf((var < 0.0f ? 0.0f : var) + eps);   // (a NaN stays one)
+    }
+};
+
 template <typename T, int TPR, int NV, bool WIDE, bool TINY>
 __global__ __launch_bounds__(WIDE ? 1024 : 256) void layernorm_kernel(const T *__restrict__ x, int64_t x_stride, int64_t M, int C,
                                                           const void *__restrict__ weight, const void *__restrict__ bias,
@@ -79,7 +99,7 @@ __global__ __launch_bounds__(WIDE ? 1024 : 256) void layernorm_kernel(const T *_
                                                           float *__restrict__ mean, float *__restrict__ rstd, int waves, int64_t per) {
     constexpr int VEC = Row<T>::VEC;
     constexpr bool HOIST = NV * VEC <= 8;                     // the weights stay in registers from row to row
-    __shared__ float red[WIDE ? 2 * MAX_WAVES : 1];
+    __shared__ float red[WIDE ? 2 * 2 * MAX_WAVES : 1];
     int slot = 0;
     const Lanes<TPR, WIDE> at_row(waves);                     // (WIDE: one row a workgroup)
     const int lane = at_row.lane, width = at_row.width;
@@ -96,37 +116,39 @@ __global__ __launch_bounds__(WIDE ? 1024 : 256) void layernorm_kernel(const T *_
     }
     const int64_t begin = (int64_t)blockIdx.x * per * rows, end = begin + per * rows < M ? begin + per * rows : M;
     for (int64_t row = begin + at_row.group; row < end; row += rows) {
-        float v[NV][VEC], s[1] = {0.0f};
+        float v[NV][VEC], s[1] = {0.0f}, t[2] = {0.0f, 0.0f};
         Row<T> p[NV];
 #pragma unroll
         for (int i = 0; i < NV; ++i)
             p[i] = nerf::load_piece<TINY>(x + row * x_stride, nerf::Place<T, TINY>((i * width + lane) * VEC, C));
+        const float x0 = first_value(x + row * x_stride);
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const nerf::Place<T, TINY> at((i * width + lane) * VEC, C);
 #pragma unroll
             for (int j = 0; j < VEC; ++j) {
                 v[i][j] = (float)p[i].v[j];
-                s[0] += at.own(j) ? v[i][j] : 0.0f;
+                s[0] += at.own(j) ? v[i][j] - x0 : 0.0f;
             }
         }
         row_sum<TPR, WIDE, 1>(s, red, slot, waves);
-        const float mu = s[0] * inv_c;
-        s[0] = 0.0f;
+        const float m = fmaf(s[0], inv_c, x0);
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const nerf::Place<T, TINY> at((i * width + lane) * VEC, C);
 #pragma unroll
             for (int j = 0; j < VEC; ++j) {
-                v[i][j] -= mu;
+                v[i][j] -= m;
                 const float d = at.own(j) ? v[i][j] : 0.0f;
-                s[0] = fmaf(d, d, s[0]);
+                t[0] += d;
+                t[1] = fmaf(d, d, t[1]);
             }
         }
-        row_sum<TPR, WIDE, 1>(s, red, slot, waves);
-        const float r = 1.0f / sqrtf(s[0] * inv_c + eps);
+        row_sum<TPR, WIDE, 2>(t, red, slot, waves);
+        const Moments stat(t, inv_c, eps);
+        const float r = stat.r, shift = -stat.e * r;
         if (lane == 0) {
-            if (mean) mean[row] = mu;
+            if (mean) mean[row] = m + stat.e;
             if (rstd) rstd[row] = r;
         }
 #pragma unroll
@@ -138,7 +160,7 @@ __global__ __launch_bounds__(WIDE ? 1024 : 256) void layernorm_kernel(const T *_
             }
             Row<T> o;
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) o.v[j] = (T)fmaf(v[i][j] * r, w[HOIST ? i : 0][j], b[HOIST ? i : 0][j]);
+            for (int j = 0; j < VEC; ++j) o.v[j] = (T)fmaf(fmaf(v[i][j], r, shift), w[HOIST ? i : 0][j], b[HOIST ? i : 0][j]);
             nerf::store_piece<TINY>(y + row * C, at, o);
         }
     }
@@ -152,34 +174,36 @@ __global__ __launch_bounds__(1024) void layernorm_long_kernel(const T *__restric
                                                               T *__restrict__ y, float *__restrict__ mean,
                                                               float *__restrict__ rstd) {
     constexpr int VEC = Row<T>::VEC;
-    __shared__ float red[2 * 16];
+    __shared__ float red[2 * 2 * MAX_WAVES];
     int slot = 0;
     const float inv_c = (float)(1.0 / (double)C);
     for (int64_t row = blockIdx.x; row < M; row += gridDim.x) {
         const T *xr = x + row * x_stride;
-        float s[1] = {0.0f};
+        const float x0 = first_value(xr);
+        float s[1] = {0.0f}, t[2] = {0.0f, 0.0f};
         for (int a = threadIdx.x * VEC; a < C; a += 1024 * VEC) {
             const nerf::Place<T, false> at(a, C);
             const Row<T> p = nerf::load_piece<false>(xr, at);
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) s[0] += at.own(j) ? (float)p.v[j] : 0.0f;
+            for (int j = 0; j < VEC; ++j) s[0] += at.own(j) ? (float)p.v[j] - x0 : 0.0f;
         }
         row_sum<WAVE, true, 1>(s, red, slot, MAX_WAVES);
-        const float mu = s[0] * inv_c;
-        s[0] = 0.0f;
+        const float m = fmaf(s[0], inv_c, x0);
         for (int a = threadIdx.x * VEC; a < C; a += 1024 * VEC) {
             const nerf::Place<T, false> at(a, C);
             const Row<T> p = nerf::load_piece<false>(xr, at);
 #pragma unroll
             for (int j = 0; j < VEC; ++j) {
-                const float d = at.own(j) ? (float)p.v[j] - mu : 0.0f;
-                s[0] = fmaf(d, d, s[0]);
+                const float d = at.own(j) ? (float)p.v[j] - m : 0.0f;
+                t[0] += d;
+                t[1] = fmaf(d, d, t[1]);
             }
         }
-        row_sum<WAVE, true, 1>(s, red, slot, MAX_WAVES);
-        const float r = 1.0f / sqrtf(s[0] * inv_c + eps);
+        row_sum<WAVE, true, 2>(t, red, slot, MAX_WAVES);
+        const Moments stat(t, inv_c, eps);
+        const float r = stat.r, shift = -stat.e * r;
         if (threadIdx.x == 0) {
-            if (mean) mean[row] = mu;
+            if (mean) mean[row] = m + stat.e;
             if (rstd) rstd[row] = r;
         }
         for (int a = threadIdx.x * VEC; a < C; a += 1024 * VEC) {
@@ -190,7 +214,7 @@ __global__ __launch_bounds__(1024) void layernorm_long_kernel(const T *__restric
             nerf::load_weights<false, T>(bias, w_f32, at, 0.0f, b);
             Row<T> o;
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) o.v[j] = (T)fmaf(((float)p.v[j] - mu) * r, w[j], b[j]);
+            for (int j = 0; j < VEC; ++j) o.v[j] = (T)fmaf(fmaf((float)p.v[j] - m, r, shift), w[j], b[j]);
             nerf::store_piece<false>(y + row * C, at, o);
         }
     }
