@@ -1,5 +1,6 @@
 """Learned-code operators (embedding, layer norm, dropout): what they refuse, before anything touches a GPU."""
 import ctypes
+import itertools
 
 import pytest
 import torch
@@ -120,3 +121,14 @@ def test_functions_and_modules_refuse_before_the_backward_pass_would():
         with pytest.raises(ValueError, match="residual"):
             drop(x, r)
     assert torch.equal(drop(x, x + 1), x + 1)
+
+
+def test_dropout_modules_without_a_seed_have_one_each(monkeypatch):
+    """Two modules of one seed would drop the same elements at every step.  The seeds repeat where a model is built again in
+    the same order, whatever explicit seeds are in between, and an explicit one is taken as it is."""
+    def build():
+        monkeypatch.setattr(layers, "_unseeded", itertools.count())
+        return [layers.Dropout(0.1).seed, layers.Dropout(0.1).seed, layers.Dropout(0.1, seed=3).seed, layers.Dropout().seed]
+    seeds = build()
+    assert len(set(seeds)) == 4 and seeds[2] == 3 and build() == seeds
+    assert layers.Dropout(0.5, 0).seed == 0 and layers.Dropout(seed=2 ** 63).seed == 2 ** 63

@@ -747,6 +747,19 @@ def test_modules_in_a_conditioned_network():
     assert drop(code) is code
 
 
+def test_default_dropout_modules_draw_masks_of_their_own():
+    """Share of elements that two modules both keep on their n-th call: (1 - p)^2 within 6 sigma, not 1 - p."""
+    n, p = 1 << 18, 0.5
+    x = torch.ones(n, device="cuda")
+    a, b = layers.Dropout(p), layers.Dropout(p)
+    for _ in range(3):
+        both = int(((a(x) != 0) & (b(x) != 0)).sum())
+        assert abs(both - n / 4) <= 6 * (n * 0.25 * 0.75) ** 0.5
+    same = layers.Dropout(p, seed=a.seed)
+    a.calls = 0
+    assert torch.equal(a(x), same(x))
+
+
 # --------------------------------------------------------------------------- streams and graphs
 def test_on_another_stream_and_two_at_once():
     g = gen(10)

@@ -6,6 +6,7 @@ train with the networks, also under ``optim.FusedAdam``.  Parameters are named a
 same names, so their state_dicts are interchangeable.  There is no CPU fallback: the modules raise for tensors off the GPU
 (a Dropout that drops nothing launches nothing, and takes any).
 """
+import itertools
 from typing import Optional
 
 import torch
@@ -51,18 +52,26 @@ class LayerNorm(nn.Module):
         return ops.LayerNormFunction.apply(x, self.weight, self.bias, self.eps)
 
 
-class Dropout(nn.Module):
-    """Counter-based dropout.  The n-th call in training mode uses key(seed, n): give every module a seed of its own, and
-    the same one on every rank (a rank passes the flat index of its first element as `first`).  Inside a graph capture the
-    count would be frozen into the graph: pass a key tensor there.  A forward that is run again for its gradient (activation
-    checkpointing) would count twice and draw another mask: pass a key there, too.  The count (`calls`) is not part of the
-    state_dict, whose keys are torch.nn.Dropout's (none): a resumed run sets it."""
+_unseeded = itertools.count()            # Dropout modules made without a seed in this process
 
-    def __init__(self, p: float = 0.5, seed: int = 0):
+
+class Dropout(nn.Module):
+    """Counter-based dropout.  The n-th call in training mode uses key(seed, n).  Modules of one seed drop the same elements, so
+    each has its own: without `seed`, one that follows from how many modules were made without one before, the same on
+    every rank that builds its model in the same order (a rank passes the flat index of its first element as `first`); a
+    program whose ranks or runs build differently names its seeds.  A copy of a module keeps its seed.
+
+    Inside a graph capture the count would be frozen into the graph: pass a key tensor there.  A forward that is run again for
+    its gradient (activation checkpointing) would count twice and draw another mask: pass a key there, too.  The count
+    (`calls`) is not part of the state_dict, whose keys are torch.nn.Dropout's (none): a resumed run sets it."""
+
+    def __init__(self, p: float = 0.5, seed: Optional[int] = None):
         super().__init__()
         if not 0.0 <= p <= 1.0:
             raise ValueError(f"dropout: p must be in [0, 1], got {p}")
-        self.p, self.seed, self.calls = float(p), int(seed), 0
+        # (mixed, so that it is not one of the small numbers that a program would name)
+        self.seed = _mix_int(next(_unseeded) ^ 0x5851F42D4C957F2D) if seed is None else int(seed)
+        self.p, self.calls = float(p), 0
 
     def forward(self, x: torch.Tensor, residual: Optional[torch.Tensor] = None, first: int = 0, key=None) -> torch.Tensor:
         if not self.training or self.p == 0.0:
