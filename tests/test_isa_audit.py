@@ -40,3 +40,20 @@ def test_no_kernel_spills_beyond_its_allowance(audit_output):
     lines = [ln for ln in audit_output.splitlines() if ln.startswith("scratch audit:")]
     assert len(lines) == 1 and lines[0].endswith("0 over their allowance"), audit_output[-2000:]
     assert int(lines[0].split()[2]) >= 60                         # every kernel of the five files was looked at
+
+
+def test_every_kernel_file_is_audited(audit_output):
+    files = sorted(f[:-4] for f in os.listdir(CSRC) if f.endswith(".hip"))
+    assert len(files) >= 17
+    for name in files:
+        assert f"build/{name}.s: " in audit_output, name
+
+
+@pytest.mark.parametrize("line,bad", [("v_pk_fma_f32 v[0:1], v[2:3], v[4:5], v[0:1]", True), ("v_pk_mul_f32 v[0:1], v[2:3], s[4:5]", True),
+                                      ("v_pk_add_f32 v[0:1], v[2:3], v[4:5] op_sel_hi:[1,0]", True),
+                                      ("v_pk_add_f16 v0, v1, v2", False), ("v_fma_f32 v0, v1, v2, v3", False)])
+def test_packed_fp32_instructions_fail_the_audit(tmp_path, line, bad):
+    path = tmp_path / "k.s"
+    path.write_text(f"_Z1kv:\n\ts_mov_b32 s0, 0\n\t{line}\n\ts_endpgm\n")
+    out = subprocess.run(["python3", os.path.join(ROOT, "scripts", "audit_asm_loads.py"), str(path)], capture_output=True, text=True)
+    assert out.returncode == int(bad) and ("packed fp32" in out.stdout) == bad, out.stdout + out.stderr
