@@ -57,3 +57,29 @@ def test_packed_fp32_instructions_fail_the_audit(tmp_path, line, bad):
     path.write_text(f"_Z1kv:\n\ts_mov_b32 s0, 0\n\t{line}\n\ts_endpgm\n")
     out = subprocess.run(["python3", os.path.join(ROOT, "scripts", "audit_asm_loads.py"), str(path)], capture_output=True, text=True)
     assert out.returncode == int(bad) and ("packed fp32" in out.stdout) == bad, out.stdout + out.stderr
+
+
+def test_a_variant_of_one_file_is_built_with_the_regular_flags(tmp_path):
+    """scripts/variant_one_file.sh, with a compiler that only writes down its arguments: the flags of the regular build
+    (`make -n`) and the extra define."""
+    log, fake = tmp_path / "log", tmp_path / "hipcc"
+    fake.write_text(f'#!/bin/bash\necho "$@" >> {log}\nwhile [ $# -gt 1 ]; do [ "$1" = -o ] && : > "$2"; shift; done\n')
+    fake.chmod(0o755)
+    name = f"test{os.getpid()}"
+    made = [os.path.join(CSRC, f"build_{name}", "adam.hip.o"), os.path.join(CSRC, "..", "lib", "variants", f"{name}.so")]
+    env = {**os.environ, "HIPCC": str(fake)}
+    try:
+        out = subprocess.run(["bash", os.path.join(ROOT, "scripts", "variant_one_file.sh"), name, "adam.hip", "-DX_TEST=1"],
+                             env=env, capture_output=True, text=True)
+        assert out.returncode == 0 and all(os.path.exists(m) for m in made), out.stdout + out.stderr
+    finally:
+        for m in made:
+            if os.path.exists(m):
+                os.remove(m)
+        if os.path.isdir(os.path.dirname(made[0])):
+            os.rmdir(os.path.dirname(made[0]))
+    plain = subprocess.run(["make", "-C", CSRC, "-nB", "build/adam.hip.o"], env=env, capture_output=True, text=True).stdout
+    regular = next(ln for ln in plain.splitlines() if " -c adam.hip" in ln).split(" -c ")[0].split()[1:]
+    compiled, linked = log.read_text().splitlines()
+    assert compiled.split(" -c ")[0].split() == regular + ["-DX_TEST=1"] and "-packed-fp32-ops" in regular
+    assert "build/adam.hip.o" not in linked.split() and f"build_{name}/adam.hip.o" in linked
