@@ -261,6 +261,32 @@ def test_layernorm_of_the_lowest_value(t, C):
     assert torch.equal(y[0], clean[0]) and torch.equal(y[3], clean[3])
 
 
+def odd(g, *shape, t=F32):
+    """-3, -1, 1 or 3: products and sums of them are whole numbers, and none is 0."""
+    return (2 * torch.randint(-1, 3, shape, generator=g) - 1).to(t).cuda()
+
+
+# rows that every way of the backward pass takes: one workgroup, striding, the order of the addresses, several wavefronts a row
+# (one and more rows a workgroup), longer than a workgroup's registers
+WALKS = [(5, 3), (4097, 3), (3, 130), (9001, 20), (20011, 32), (262145, 130), (300000, 256), (70, 512), (5000, 600), (2000, 1030),
+         (1500, 4100), (700, 9000), (1030, 16000), (130, 20011)]
+
+
+@pytest.mark.parametrize("t", DTYPES)
+@pytest.mark.parametrize("M,C", WALKS)
+def test_layernorm_column_sums_count_every_row_once(t, M, C):
+    """The backward pass takes mean and rstd as they are given: with mean 0 and rstd 1 the weight's gradient is the sum of
+    g x, the bias's that of g.  Of small odd numbers both are whole numbers below 9 M < 2^24, exact in fp32 in any order, and
+    a row that is left out or counted twice changes every column."""
+    assert 9 * M < 2 ** 24
+    g = gen(M + C)
+    x, go, w = odd(g, M, C, t=t), odd(g, M, C, t=t), torch.ones(C, device="cuda")
+    gx, gw, gb = ops.layernorm_backward(go, x, w, torch.zeros(M, device="cuda"), torch.ones(M, device="cuda"))
+    assert torch.equal(gw.double(), (go.double() * x.double()).sum(0)) and torch.equal(gb.double(), go.double().sum(0))
+    few = ops.layernorm_backward(go, x, w.to(t), torch.zeros(M, device="cuda"), torch.ones(M, device="cuda"))
+    assert torch.equal(few[1], gw.to(t)) and torch.equal(few[2], gb.to(t)) and torch.equal(few[0], gx)
+
+
 def test_layernorm_infinities_and_nans_stay_in_their_rows():
     g = gen(3)
     x = randn(g, 9, 70)
@@ -386,6 +412,23 @@ def test_embedding_and_its_gradient(t, n, rows, dim):
         tol = U * want.abs()
         close(out, want, tol + half(t) * (want.abs() + tol) + step0(t), kind)
         check_embedding_backward(randn(g, n, dim, t=t), ids, rows, scale, pad, what=f"{kind} {n} {rows} {dim} {t}")
+
+
+@pytest.mark.parametrize("t", DTYPES)
+@pytest.mark.parametrize("n,rows,dim", [(786432, 100, 48), (786432, 1, 20), (786432, 255, 5), (300000, 1000, 33), (300000, 2000, 7),
+                                        (32768, 300, 1100), (20000, 90000, 9), (1000, 4000, 600), (70000, 3, 1030)])
+def test_embedding_gradient_counts_every_row_once(n, rows, dim, t):
+    """Sums of small odd numbers are whole numbers below 3 n < 2^24, exact in fp32 in any order: what comes back is the exact
+    sum, rounded once, and a row that is left out or counted twice changes every value of its id.  One id per run of 192
+    (a ray's samples), ids that differ from sample to sample, and one id for all."""
+    assert 3 * n < 2 ** 24
+    g = gen(n + dim)
+    go = odd(g, n, dim, t=t)
+    rays = torch.randint(rows, ((n + 191) // 192,), generator=g).repeat_interleave(192)[:n]
+    for ids in (rays, torch.randint(rows, (n,), generator=g), torch.full((n,), rows - 1)):
+        got = ops.embedding_backward(go, ids.cuda(), rows)
+        want = torch.zeros(rows, dim, dtype=torch.int32).index_add_(0, ids, go.to(torch.int32).cpu())
+        assert torch.equal(got.cpu(), want.double().to(t))
 
 
 def test_embedding_scale_one_is_a_copy():
