@@ -287,6 +287,53 @@ def test_layernorm_column_sums_count_every_row_once(t, M, C):
     assert torch.equal(few[1], gw.to(t)) and torch.equal(few[2], gb.to(t)) and torch.equal(few[0], gx)
 
 
+@pytest.mark.parametrize("t", [F32, BF16])
+@pytest.mark.parametrize("M,C", WALKS)
+def test_layernorm_of_a_matrix_columns(t, M, C):
+    """x and g as columns of wider matrices, of two widths, at odd offsets, and as every second row: the same bits as their
+    copies give, forward and backward, in every kind of row."""
+    g = gen(M + C)
+    xs = torch.randn(M, C + 37, device="cuda").to(t)[:, 5:5 + C]
+    gs = torch.randn(M, C + 12, device="cuda").to(t)[:, 3:3 + C]
+    w, b = randn(g, C, t=t), randn(g, C, t=t)
+    for x, go in ((xs, gs), (xs, gs.contiguous()), (xs[::2], gs[::2])):
+        got = ops.layernorm(x, w, b, want_stats=True)
+        want = ops.layernorm(x.contiguous(), w, b, want_stats=True)
+        assert all(torch.equal(a, c) for a, c in zip(got, want))
+        got = ops.layernorm_backward(go, x, w, *got[1:])
+        want = ops.layernorm_backward(go.contiguous(), x.contiguous(), w, *want[1:])
+        assert all(torch.equal(a, c) for a, c in zip(got, want))
+
+
+@pytest.mark.parametrize("t", DTYPES)
+@pytest.mark.parametrize("M,C", [(9, 3), (9, 20), (9, 300), (9, 600), (9, 3000), (9, 9000), (9, 20011), (1100, 5), (1100, 130),
+                                 (1100, 1030), (1100, 9000)])
+def test_layernorm_infinities_and_nans_in_every_kind_of_row(t, M, C):
+    """A value that is not finite, at the row's first, last or an inner place, makes its own row of y and of g_x NaN or
+    infinite and no other; in g it reaches its column's sums, in x all of the weight's and none of the bias's."""
+    g = gen(C)
+    x, go, w, b = randn(g, M, C, t=t), randn(g, M, C, t=t), randn(g, C, t=t), randn(g, C, t=t)
+    y0, mu0, r0 = ops.layernorm(x, w, b, want_stats=True)
+    gx0, gw0, gb0 = ops.layernorm_backward(go, x, w, mu0, r0)
+    xb = x.clone()
+    xb[2, 0], xb[4, C - 1], xb[M - 2, C // 2] = float("inf"), float("nan"), -float("inf")
+    bad = torch.zeros(M, dtype=torch.bool, device="cuda")
+    bad[[2, 4, M - 2]] = True
+    y, mu, r = ops.layernorm(xb, w, b, want_stats=True)
+    assert torch.equal(y[~bad], y0[~bad]) and torch.equal(mu[~bad], mu0[~bad]) and torch.equal(r[~bad], r0[~bad])
+    assert bool(y[bad].isnan().any(1).all()) and bool(r[bad].isnan().all()) and not bool(mu[bad].isfinite().any())
+    gx, gw, gb = ops.layernorm_backward(go, xb, w, mu, r)
+    assert torch.equal(gx[~bad], gx0[~bad]) and not bool(gx[bad].isfinite().any())
+    assert bool(gw.isnan().all()) and torch.equal(gb, gb0)
+    gbad = go.clone()
+    gbad[3, C - 1] = float("inf")
+    gx, gw, gb = ops.layernorm_backward(gbad, x, w, mu0, r0)
+    rest = torch.arange(M, device="cuda") != 3
+    assert torch.equal(gx[rest], gx0[rest]) and not bool(gx[3].isfinite().any())
+    assert torch.equal(gb[:-1], gb0[:-1]) and not bool(gb[-1].isfinite()) and torch.equal(gw[:-1], gw0[:-1])
+    assert not bool(gw[-1].isfinite())
+
+
 def test_layernorm_infinities_and_nans_stay_in_their_rows():
     g = gen(3)
     x = randn(g, 9, 70)
