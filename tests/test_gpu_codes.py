@@ -200,8 +200,10 @@ def check_norm_offset(x, w, b, eps=1e-5, what=""):
     """y, mean and rstd with bounds that an offset common to a row's values does not widen, but for the one rounding of a
     mean that is stored as fp32.
 
-    With u = x - x0 (rounded: U |u|), k additions on a term's way: the first mean m is off by at most delta =
-    U |mu| + (k + 3) U mean|u|.  d = x - m is off by U |d|, |d| <= D = |x - mu| + delta; e = mean(d) by (k + 3) U A, A = mean D.
+    Let k be the additions on a term's way.  The mean m that the deviations are summed about is off by delta: its own rounding
+    U |mu|, and (k + 3) U mean|u| for a sum of numbers of the deviations' size, u = x - x0.  (Where m is less than 2^10
+    deviations it may be the plain mean, off by 2^-9 of a deviation at most: 0.2 % of what follows, in bounds that count
+    every rounding at its largest.)  d = x - m is off by U |d|, |d| <= D = |x - mu| + delta; e = mean(d) by (k + 3) U A, A = mean D.
     So the numerator x - m - e is off by U D + (k + 5) U A (the last two: the product e r).  The variance mean(d^2) - e^2 is
     off by (k + 6) U (V + delta^2) + 2 (delta + (k + 3) U A) (k + 3) U A + U delta^2, where V is the exact one; 1 / sqrt
     takes half of that relative to V + eps (0.75 with the higher orders, below 0.2) and 4 roundings."""

@@ -4,11 +4,12 @@
 //   gx = r (q - mean(q) - h mean(q h)),  q = g w, h = (x - mu) r;   gw = sum_rows g h,   gb = sum_rows g
 //
 // A row stays in registers between its one read and its one write: TPR lanes hold it as NV 16-byte pieces each.  Statistics
-// and sums are fp32, and an offset of the row costs no digits: a plain sum of x would be off by some roundings of the
-// offset's size, which may be larger than the deviations.  So the first sum is of x - x0, x0 the row's first value, which
-// gives m, a mean to within about a rounding, and the second sums are of d = x - m and of d^2; with e = mean(d)
+// and sums are fp32, and an offset of the row costs no digits.  The first mean m, from the sum of x, is off by some roundings
+// of the offset's size, which may be larger than the deviations; the second sums are of d = x - m and of d^2, and with e = mean(d)
 //   mu = m + e,   var = mean(d^2) - e^2,   (x - mu) r = d r - e r
-// are off by roundings of the deviations' size.  (mu itself is stored as fp32, and that is what the backward pass takes.)
+// are off by roundings of the deviations' size.  Where m is smaller than the deviations it is no worse than m + e, and e is
+// taken as 0.  Where it is so much larger that e^2 is not small beside var (constant rows), d - e is summed once more in
+// place of d.  (mu itself is stored as fp32, and that is what the backward pass takes.)
 // Rows of up to 64 lanes need no barrier; a longer row takes several wavefronts.
 //
 // Bound by HBM.  Forward 262144 x 256 fp32: 90 us, 6.0 TB/s read + written (a copy of that size: 5.4); 16384 x 2048 bf16
@@ -35,7 +36,8 @@ __device__ __forceinline__ void row_sum(float (&v)[K], float *red, int &slot, in
     for (int k = 0; k < K; ++k) v[k] = nerf::lane_sum<TPR>(v[k]);
     if constexpr (WIDE) {
         const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
-        float *r = red + slot * MAX_WAVES * K;
+        float *r = red + slot * 2 * MAX_WAVES;                // (the same halves for one value and for two)
+        static_assert(K <= 2, "red");
         slot ^= 1;
         if ((threadIdx.x & (WAVE - 1)) == 0) {
 #pragma unroll
@@ -76,21 +78,20 @@ __device__ __forceinline__ void forget(Row<T> &p) {
     __builtin_memcpy(&p, u, 16);
 }
 
-// x0.  0 in place of a value so large that a sum of C differences from it could overflow where the values' own does not.
-template <typename T>
-__device__ __forceinline__ float first_value(const T *row) {
-    const float v = (float)row[0];
-    return fabsf(v) < 1e30f ? v : 0.0f;
-}
-
-// From the sums of d and of d^2, d = x - m with a first mean m: e, the mean of d, and r.
+// From the sums of d and of d^2, d = x - m: e = mean(d) where that improves m, and r.  (A NaN stays one, an infinity too.)
 struct Moments {
     float e, r;
-    __device__ __forceinline__ Moments(const float (&sums)[2], float inv_c, float eps) : e(sums[0] * inv_c) {
-        const float var = fmaf(-e, e, sums[1] * inv_c);
-        r = 1.0f / sqrtf((var < 0.0f ? 0.0f : var) + eps);   // (a NaN stays one)
+    __device__ __forceinline__ Moments(const float (&sums)[2], float m, float inv_c, float eps) {
+        const float square = sums[1] * inv_c;
+        e = m * m > square ? sums[0] * inv_c : 0.0f;
+        const float var = fmaf(-e, e, square);
+        r = 1.0f / sqrtf((var < 0.0f ? 0.0f : var) + eps);
     }
 };
+
+// The sums are to be taken again, about m + e: m is 2^10 deviations or more.  (28 roundings take m off by 2^-19 of itself, by 2^-9
+// of a deviation where this says no: e^2 is 2^-18 of the variance.)  The same for all lanes that share a row.
+__device__ __forceinline__ bool far_off(const float (&sums)[2], float m, float inv_c) { return m * m > 0x1p20f * (sums[1] * inv_c); }
 
 template <typename T, int TPR, int NV, bool WIDE, bool TINY>
 __global__ __launch_bounds__(WIDE ? 1024 : 256) void layernorm_kernel(const T *__restrict__ x, int64_t x_stride, int64_t M, int C,
@@ -116,36 +117,44 @@ __global__ __launch_bounds__(WIDE ? 1024 : 256) void layernorm_kernel(const T *_
     }
     const int64_t begin = (int64_t)blockIdx.x * per * rows, end = begin + per * rows < M ? begin + per * rows : M;
     for (int64_t row = begin + at_row.group; row < end; row += rows) {
-        float v[NV][VEC], s[1] = {0.0f}, t[2] = {0.0f, 0.0f};
+        float v[NV][VEC], s[1] = {0.0f}, t[2];
         Row<T> p[NV];
 #pragma unroll
         for (int i = 0; i < NV; ++i)
             p[i] = nerf::load_piece<TINY>(x + row * x_stride, nerf::Place<T, TINY>((i * width + lane) * VEC, C));
-        const float x0 = first_value(x + row * x_stride);
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const nerf::Place<T, TINY> at((i * width + lane) * VEC, C);
 #pragma unroll
             for (int j = 0; j < VEC; ++j) {
                 v[i][j] = (float)p[i].v[j];
-                s[0] += at.own(j) ? v[i][j] - x0 : 0.0f;
+                s[0] += at.own(j) ? v[i][j] : 0.0f;
             }
         }
         row_sum<TPR, WIDE, 1>(s, red, slot, waves);
-        const float m = fmaf(s[0], inv_c, x0);
+        float m = s[0] * inv_c;
+        auto about = [&](float shift) {                       // v -= shift; t <- the sums of v and v^2
+            t[0] = t[1] = 0.0f;
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const nerf::Place<T, TINY> at((i * width + lane) * VEC, C);
+            for (int i = 0; i < NV; ++i) {
+                const nerf::Place<T, TINY> at((i * width + lane) * VEC, C);
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) {
-                v[i][j] -= m;
-                const float d = at.own(j) ? v[i][j] : 0.0f;
-                t[0] += d;
-                t[1] = fmaf(d, d, t[1]);
+                for (int j = 0; j < VEC; ++j) {
+                    v[i][j] -= shift;
+                    const float d = at.own(j) ? v[i][j] : 0.0f;
+                    t[0] += d;
+                    t[1] = fmaf(d, d, t[1]);
+                }
             }
+            row_sum<TPR, WIDE, 2>(t, red, slot, waves);
+        };
+        about(m);
+        if (far_off(t, m, inv_c)) {
+            const float e = t[0] * inv_c;
+            m += e;
+            about(e);
         }
-        row_sum<TPR, WIDE, 2>(t, red, slot, waves);
-        const Moments stat(t, inv_c, eps);
+        const Moments stat(t, m, inv_c, eps);
         const float r = stat.r, shift = -stat.e * r;
         if (lane == 0) {
             if (mean) mean[row] = m + stat.e;
@@ -179,31 +188,39 @@ __global__ __launch_bounds__(1024) void layernorm_long_kernel(const T *__restric
     const float inv_c = (float)(1.0 / (double)C);
     for (int64_t row = blockIdx.x; row < M; row += gridDim.x) {
         const T *xr = x + row * x_stride;
-        const float x0 = first_value(xr);
-        float s[1] = {0.0f}, t[2] = {0.0f, 0.0f};
+        float s[1] = {0.0f}, t[2];
         for (int a = threadIdx.x * VEC; a < C; a += 1024 * VEC) {
             const nerf::Place<T, false> at(a, C);
             const Row<T> p = nerf::load_piece<false>(xr, at);
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) s[0] += at.own(j) ? (float)p.v[j] - x0 : 0.0f;
+            for (int j = 0; j < VEC; ++j) s[0] += at.own(j) ? (float)p.v[j] : 0.0f;
         }
         row_sum<WAVE, true, 1>(s, red, slot, MAX_WAVES);
-        const float m = fmaf(s[0], inv_c, x0);
-        for (int a = threadIdx.x * VEC; a < C; a += 1024 * VEC) {
-            const nerf::Place<T, false> at(a, C);
-            const Row<T> p = nerf::load_piece<false>(xr, at);
+        const float m = s[0] * inv_c;
+        float e = 0.0f;
+        auto about = [&] {                                    // t <- the sums of d = x - m - e and of d^2
+            t[0] = t[1] = 0.0f;
+            for (int a = threadIdx.x * VEC; a < C; a += 1024 * VEC) {
+                const nerf::Place<T, false> at(a, C);
+                const Row<T> p = nerf::load_piece<false>(xr, at);
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) {
-                const float d = at.own(j) ? (float)p.v[j] - m : 0.0f;
-                t[0] += d;
-                t[1] = fmaf(d, d, t[1]);
+                for (int j = 0; j < VEC; ++j) {
+                    const float d = at.own(j) ? ((float)p.v[j] - m) - e : 0.0f;
+                    t[0] += d;
+                    t[1] = fmaf(d, d, t[1]);
+                }
             }
+            row_sum<WAVE, true, 2>(t, red, slot, MAX_WAVES);
+        };
+        about();
+        if (far_off(t, m, inv_c)) {
+            e = t[0] * inv_c;
+            about();
         }
-        row_sum<WAVE, true, 2>(t, red, slot, MAX_WAVES);
-        const Moments stat(t, inv_c, eps);
+        const Moments stat(t, m, inv_c, eps);
         const float r = stat.r, shift = -stat.e * r;
         if (threadIdx.x == 0) {
-            if (mean) mean[row] = m + stat.e;
+            if (mean) mean[row] = m + (e + stat.e);
             if (rstd) rstd[row] = r;
         }
         for (int a = threadIdx.x * VEC; a < C; a += 1024 * VEC) {
@@ -214,7 +231,7 @@ __global__ __launch_bounds__(1024) void layernorm_long_kernel(const T *__restric
             nerf::load_weights<false, T>(bias, w_f32, at, 0.0f, b);
             Row<T> o;
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) o.v[j] = (T)fmaf(fmaf((float)p.v[j] - m, r, shift), w[j], b[j]);
+            for (int j = 0; j < VEC; ++j) o.v[j] = (T)fmaf(fmaf(((float)p.v[j] - m) - e, r, shift), w[j], b[j]);
             nerf::store_piece<false>(y + row * C, at, o);
         }
     }
