@@ -298,8 +298,10 @@ enum { NERF_F32 = 0, NERF_BF16 = 1, NERF_F16 = 2 };
  * [0, rows) is not dereferenced: its row is NaN. */
 int nerf_embedding(const void *table, int64_t rows, int64_t row_stride, int dtype, int64_t dim, const void *ids,
                    int id_bytes, int64_t n, float scale, void *out, nerf_stream_t stream);
-/* g_table (rows,dim), OVERWRITTEN: scale * the sum of the rows of g_out (n,dim) by id, in the order of the batch; rows
- * that no id names are 0.  Ids outside [0, rows) and ids equal to padding_idx (< 0: none) give nothing.
+/* g_table (rows,dim), OVERWRITTEN: scale * the sum of the rows of g_out (n,dim) by id; rows that no id names are 0.  The order
+ * of a sum follows from the ids, the sizes and the dtype alone (short runs in the order of the batch, then their sums in
+ * interleaved groups): the same call gives the same bits.  Ids outside [0, rows) and ids equal to padding_idx (< 0: none)
+ * give nothing.
  * workspace: nerf_embedding_backward_workspace_bytes; n < 2^31, rows < 2^31, dim <= 2^20. */
 int64_t nerf_embedding_backward_workspace_bytes(int64_t n, int64_t rows, int64_t dim, int dtype);
 int nerf_embedding_backward(const void *g_out, int dtype, int64_t n, int64_t dim, const void *ids, int id_bytes,
@@ -307,7 +309,8 @@ int nerf_embedding_backward(const void *g_out, int dtype, int64_t n, int64_t dim
                             nerf_stream_t stream);
 
 /* y (M,C) = (x - mean) * rstd * weight + bias over rows of x (M,C), x_stride; mean, rstd (M,) fp32 may be NULL, weight and
- * bias (C,) of w_dtype (dtype or fp32) may be NULL. */
+ * bias (C,) of w_dtype (dtype or fp32) may be NULL.  An offset common to a row's values costs y and rstd no digits; the mean is
+ * rounded to fp32 when it is stored, and that is the mean which the backward pass subtracts. */
 int nerf_layernorm(const void *x, int64_t x_stride, int dtype, int64_t M, int64_t C, const void *weight, const void *bias,
                    int w_dtype, double eps, void *y, float *mean, float *rstd, nerf_stream_t stream);
 /* g_x (M,C) and, when non-NULL, g_weight / g_bias (C,) of w_dtype, all OVERWRITTEN; mean, rstd as the forward left them.

@@ -13,10 +13,15 @@
 // Rows of up to 64 lanes need no barrier; a longer row takes several wavefronts.
 //
 // Bound by HBM.  Forward 262144 x 256 fp32: 90 us, 6.0 TB/s read + written (a copy of that size: 5.4); 16384 x 2048 bf16
-// 26 us (5.1); 1 row of 4096: 2.6 us.  Backward 786432 x 256 fp32: 453 + 12 us for the columns, 5.2 TB/s; 8192 x 4096 bf16:
-// 41 + 5 us, 4.4 TB/s.  Where it is not: rows of 8193..16384 values (a workgroup holds one row, in lockstep: 8192 x 4096
-// values as 2048 x 16384 bf16 take 79 us backward instead of 41), and rows of fewer than 8 16-bit or 4 fp32 values (value by
-// value).
+// 28 us (4.8); 8192 x 4096 fp32 46 us (5.8); 1 row of 4096: 2.8 us.  Backward 786432 x 256 fp32: 455 + 12 us for the columns,
+// 5.2 TB/s; 8192 x 4096 bf16: 40 + 5 us, 4.5 TB/s.  Where it is not:
+// - rows of 8193..16384 values: a workgroup holds one row, in lockstep.  As 2048 x 16384 bf16 the values of 8192 x 4096 take 35 us
+//   forward instead of 26 and 66 + 13 backward instead of 40 + 5 (fp32: 62 instead of 46, 105 + 13 instead of 76 + 5, with 9
+//   registers spilled);
+// - longer rows, which are read three times by one workgroup each: 1024 x 32768 36 us forward and 54 + 25 + 10 backward in bf16,
+//   83 and 100 + 48 + 10 in fp32; few and very long ones do not fill the chip (256 x 131072 fp32: 99 and 110 + 54 + 38 us);
+// - rows of fewer than 8 16-bit or 4 fp32 values, which go value by value: 11000000 x 3 fp32 76 us forward (3.5 TB/s) and 103 + 5
+//   backward (3.7), 4800000 x 7 bf16 76 (1.8) and 101 + 5 (1.9).
 #include "rows.h"
 
 namespace {

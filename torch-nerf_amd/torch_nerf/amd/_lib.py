@@ -100,7 +100,7 @@ def build(force: bool = False) -> str:
 
 
 def audit() -> None:
-    """Static ISA audit of the kernels that use hand-issued LDS reads / inline-asm VMEM (make -C csrc audit)."""
+    """Static audit of the kernels' assembly: hand-issued LDS reads, inline-asm VMEM, packed fp32, scratch (make -C csrc audit)."""
     subprocess.check_call(["make", "-C", CSRC, "-j8", "audit"], stdout=subprocess.DEVNULL)
 
 

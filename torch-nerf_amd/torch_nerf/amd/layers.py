@@ -19,7 +19,8 @@ __all__ = ["Embedding", "LayerNorm", "Dropout"]
 
 
 class Embedding(nn.Module):
-    """scale * weight[ids].  Row `padding_idx` starts at 0 and gets no gradient."""
+    """scale * weight[ids].  Row `padding_idx` starts at 0 and gets no gradient.  (The third argument is the scale;
+    torch.nn.Embedding's is padding_idx.)"""
 
     def __init__(self, num_embeddings: int, embedding_dim: int, scale: float = 1.0, padding_idx: Optional[int] = None,
                  device=None, dtype=None):
