@@ -249,6 +249,29 @@ def test_layernorm_of_rows_with_an_offset(t, C):
     assert torch.equal(y, b.expand(5, C)) and torch.equal(mu, same[:, 0].float())      # constant rows: 0 to the last bit
 
 
+@pytest.mark.parametrize("t", DTYPES)
+@pytest.mark.parametrize("C", [2, 4, 9, 31, 64, 100, 128, 200, 256, 700, 3000, 20011])
+def test_layernorm_rows_with_and_without_an_offset_side_by_side(t, C):
+    """Rows that are summed once more and rows that are not, in one wavefront where the rows are short: every row has the bits
+    that it has among rows of its own kind."""
+    g = gen(C)
+    M = 1200 if C <= 256 else 30
+    x, w, b = randn(g, M, C, t=t), randn(g, C, t=t), randn(g, C, t=t)
+    far = torch.rand(M, generator=g).cuda() < 0.5
+    x[far] = (x[far].double() * 0.01 + 20000.0).to(t)
+    x[::7] = 3333.3
+    got = ops.layernorm(x, w, b, want_stats=True)
+    kinds = (far & (torch.arange(M, device="cuda") % 7 != 0), ~far & (torch.arange(M, device="cuda") % 7 != 0),
+             torch.arange(M, device="cuda") % 7 == 0)
+    for rows in kinds:
+        same = x[rows]
+        many = same.repeat(-(-M // same.shape[0]), 1)[:M]          # as many rows: the same kernel
+        want = ops.layernorm(many, w, b, want_stats=True)
+        n = min(M, same.shape[0])
+        assert all(torch.equal(a[rows], c[:n]) for a, c in zip(got, want))
+    check_norm_offset(x, w, b, what=f"{C} {t}")
+
+
 @pytest.mark.parametrize("t", [F32, BF16])
 @pytest.mark.parametrize("C", [3, 70, 3000, 20011])
 def test_layernorm_of_the_lowest_value(t, C):
