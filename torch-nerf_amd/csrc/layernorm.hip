@@ -95,7 +95,8 @@ struct Moments {
 };
 
 // The sums are to be taken again, about m + e: m is 2^10 deviations or more.  (28 roundings take m off by 2^-19 of itself, by 2^-9
-// of a deviation where this says no: e^2 is 2^-18 of the variance.)  The same for all lanes that share a row.
+// of a deviation where this says no: e^2 is 2^-18 of the variance.  A row of C > 16384 values takes C / 1024 of them more, one
+// of 2^24 up to 2^-10: e^2 is then the variance's size at the worst.)  The same for all lanes that share a row.
 __device__ __forceinline__ bool far_off(const float (&sums)[2], float m, float inv_c) { return m * m > 0x1p20f * (sums[1] * inv_c); }
 
 template <typename T, int TPR, int NV, bool WIDE, bool TINY>
